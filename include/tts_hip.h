@@ -101,6 +101,59 @@ const char *tts_plan_last_kernel(const tts_plan *plan);
  * int8-weight product tts_plan_describe_launch tells.) */
 int tts_plan_last_slices(const tts_plan *plan, int *meet);
 
+/* ---- Operators whose weights are picked per row of activations: what a decode step does beside its shared projections.  No
+ * counterpart in the reference.  They are calls of their own, without a Triton program or a plan; otherwise they behave as
+ * tts_launch: asynchronous on `stream`, whose device has to be the current one, tensors borrowed until the stream has passed the call, nothing
+ * compiled.  They allocate nothing (and so may be captured into a graph): scratch memory is the caller's, of the size that the
+ * ..._workspace function of the same arguments says, 256-byte aligned, and free for other use once the stream has passed the call;
+ * calls that may overlap in time need one each.  Every argument is checked on the host before anything is launched; what memory
+ * holds (ids) is checked on the device.  Results do not depend on the order in which workgroups run.  A call for zero tokens does nothing. */
+
+typedef enum tts_dtype { TTS_F32 = 0, TTS_F16 = 1, TTS_BF16 = 2, TTS_I8 = 3, TTS_I32 = 4 } tts_dtype;
+/* A tensor in device memory; strides in elements, entries past `rank` are not read. */
+typedef struct tts_tensor {
+  void *ptr;
+  int32_t dtype; /* tts_dtype */
+  int32_t rank;
+  int64_t shape[3];
+  int64_t stride[3];
+} tts_tensor;
+
+typedef enum tts_scoring { TTS_SOFTMAX = 0, TTS_SIGMOID = 1 } tts_scoring;
+typedef enum tts_activation { TTS_SILU = 0, TTS_GELU_TANH = 1, TTS_RELU = 2 } tts_activation;
+
+/* The router of a mixture-of-experts layer.  logits [T, E] (f32, f16, bf16; E <= 1024), bias [E] f32 or NULL, ids [T, k] i32 and
+ * weights [T, k] f32 (k <= 64) written; rows any distance apart, elements of a row neighbours.  With s = softmax or sigmoid of a
+ * row's logits, ids are the k experts of the largest s + bias (without a bias: of the largest logits, which is the same order where
+ * neither score has run into 0 or 1), in descending order, ties to the lowest expert, and weights are scale * s, divided by
+ * the sum of the chosen s if `renormalize` (0 where s is 0).  Logits of -inf are
+ * not chosen, nor is an s + bias that is -inf or NaN; where fewer than k are left, ids are -1 and weights 0.  A row that
+ * holds a NaN has weights of NaN. */
+tts_status tts_moe_route(const tts_tensor *logits, const tts_tensor *bias, int scoring, int renormalize, double scale,
+                         const tts_tensor *ids, const tts_tensor *weights, void *stream);
+
+/* The experts of a mixture-of-experts layer for a few tokens (T * k <= 4096):
+ *   out[t] = sum over j of weights[t, j] * (h Wd[e]),  h = f(x[t] Wg[e]) * (x[t] Wu[e]),  e = ids[t, j],
+ * x [T, H] f16 or bf16, ids [T, k] i32, weights [T, k] f32, w_up [E, H, 2 I] with Wg its first I columns and Wu the others, w_down
+ * [E, I, O], out [T, O] of x's type (it may be x: all of x is read before any of out is written).  Not `gated`: w_up [E, H, I], h = f(x[t] W[e]).
+ * Weights are of x's type, or i8 with s_up [E, 2 I] and s_down [E, O] f32 that multiply their columns (NULL otherwise); each matrix
+ * has stride 1 along its inputs or along its outputs.  H, I, O >= 8.  An id outside [0, E) contributes nothing; the same id
+ * twice in a row contributes twice.  Sums, h and the weighted parts are held in 32 bits. */
+tts_status tts_moe_experts_workspace(const tts_tensor *x, const tts_tensor *ids, const tts_tensor *w_up, const tts_tensor *w_down, int gated,
+                                     size_t *bytes);
+tts_status tts_moe_experts(const tts_tensor *x, const tts_tensor *ids, const tts_tensor *weights, const tts_tensor *w_up, const tts_tensor *s_up,
+                           const tts_tensor *w_down, const tts_tensor *s_down, int activation, int gated, const tts_tensor *out,
+                           void *workspace, size_t bytes, void *stream);
+
+/* Low-rank adapters of many requests:
+ *   out[t] = base[t] + scales[d] * (x[t] a[d]^T) b[d]^T,  d = ids[t];  out[t] = base[t], bit for bit, where d is not in [0, n).
+ * base and out [T, N], x [T, K], a [n, r, K], b [n, N, r], all f16 or all bf16, the last dimension with stride 1; ids [T] i32, scales [n]
+ * f32 or NULL (1); r <= 1024.  out may be base itself; otherwise it shares no memory with the inputs.  One request's adapter
+ * (an infinity in it, say) does not reach another's rows.  Rows of one adapter next to each other read it once per 16 or 64 rows. */
+tts_status tts_lora_add_workspace(const tts_tensor *x, const tts_tensor *b, size_t *bytes);
+tts_status tts_lora_add(const tts_tensor *base, const tts_tensor *x, const tts_tensor *a, const tts_tensor *b, const tts_tensor *ids,
+                        const tts_tensor *scales, const tts_tensor *out, void *workspace, size_t bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,15 @@ class TtsArg(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int32), ("reserved", ctypes.c_int32), ("v", _ArgValue)]
 
 
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8, DTYPE_I32 = 0, 1, 2, 3, 4
+
+
+class TtsTensor(ctypes.Structure):
+    """tts_tensor: a tensor in device memory, strides in elements."""
+    _fields_ = [("ptr", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("rank", ctypes.c_int32), ("shape", ctypes.c_int64 * 3),
+                ("stride", ctypes.c_int64 * 3)]
+
+
 def build(verbose=False):
     """Compiles the library in-tree with hipcc for gfx950 (cross-compiles without a GPU)."""
     cmd = ["make", "-C", _CSRC, "-j8", f"PYTHON={sys.executable}", "all"]
@@ -66,6 +75,14 @@ def lib():
     L.tts_launch.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                              ctypes.POINTER(TtsArg), ctypes.c_int]
     L.tts_launch_noalloc.argtypes = L.tts_launch.argtypes
+    t, size = ctypes.POINTER(TtsTensor), ctypes.POINTER(ctypes.c_size_t)
+    stream, flag = ctypes.c_void_p, ctypes.c_int
+    scratch = [ctypes.c_void_p, ctypes.c_size_t]
+    L.tts_moe_route.argtypes = [t, t, flag, flag, ctypes.c_double, t, t, stream]
+    L.tts_moe_experts_workspace.argtypes = [t, t, t, t, flag, size]
+    L.tts_moe_experts.argtypes = [t, t, t, t, t, t, t, flag, flag, t, *scratch, stream]
+    L.tts_lora_add_workspace.argtypes = [t, t, size]
+    L.tts_lora_add.argtypes = [t, t, t, t, t, t, t, *scratch, stream]
     _lib = L
     return L
 

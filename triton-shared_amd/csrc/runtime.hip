@@ -36,6 +36,14 @@ tts_status fail(tts_status st, const std::string &msg) {
   return st;
 }
 
+}  // namespace
+
+namespace tts {
+tts_status report(tts_status st, const std::string &msg) { return fail(st, msg); }
+}  // namespace tts
+
+namespace {
+
 char *dup_string(const std::string &s) {
   char *p = (char *)malloc(s.size() + 1);
   memcpy(p, s.c_str(), s.size() + 1);
