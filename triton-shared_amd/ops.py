@@ -40,6 +40,23 @@ def _describe(name, t, device):
     return d
 
 
+_fast = None
+
+
+def _native_calls():
+    """The launch extension's own moe_route, moe_experts and lora_add (csrc/launch_module.cpp), which take the ordinary calls; False without it."""
+    global _fast
+    module, lib = _native.launch_module(), _native.lib()
+    if module is None:
+        _fast = False
+    else:
+        address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+        module.setup_ops(address(lib.tts_moe_route), address(lib.tts_moe_experts_workspace), address(lib.tts_moe_experts), address(lib.tts_lora_add_workspace), address(lib.tts_lora_add),
+                         torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, *_DTYPES, torch.Tensor, torch.nn.Parameter, _native._raise)
+        _fast = module
+    return _fast
+
+
 def _device_of(name, t):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} is a {type(t).__name__}, not a tensor")
@@ -76,6 +93,11 @@ def moe_route(logits, k, scoring="softmax", bias=None, renormalize=True, scale=1
     largest first, ties to the lowest expert; weights are scale * s, over the sum of the chosen s if `renormalize`.  Logits of -inf are never chosen: where fewer
     than k others are left, ids are -1 and weights 0.  A row that holds a NaN gets weights of NaN.
     """
+    fast = _native_calls() if _fast is None else _fast
+    if fast:
+        made = fast.moe_route(logits, k, _SCORING.get(scoring), bias, renormalize, scale)
+        if made is not None:
+            return made
     device = _device_of("logits", logits)
     if logits.dim() != 2:
         raise ValueError(f"logits have {logits.dim()} dimensions, not 2")
@@ -98,6 +120,11 @@ def moe_experts(x, ids, weights, w_up, w_down, s_up=None, s_down=None, activatio
     Either dimension of a matrix may be the contiguous one: pass `w.transpose(1, 2)` of weights stored as [E, outputs, inputs].
     An id outside [0, E) contributes nothing.  `out` may be x.
     """
+    fast = _native_calls() if _fast is None else _fast
+    if fast:
+        made = fast.moe_experts(x, ids, weights, w_up, w_down, s_up, s_down, _ACTIVATION.get(activation), gated, out)
+        if made is not None:
+            return made
     device = _device_of("x", x)
     act = _choice("activation", activation, _ACTIVATION)
     dx, di, du, dd = _describe("x", x, device), _describe("ids", ids, device), _describe("w_up", w_up, device), _describe("w_down", w_down, device)
@@ -117,6 +144,11 @@ def lora_add(base, x, a, b, ids, scales=None, out=None):
     base [T, N], x [T, K], a [n, r, K], b [n, N, r] (as nn.Linear stores such weights), all float16 or all bfloat16; ids [T] int32, scales [n] float32
     or None for 1.  `out` may be base itself, for an update in place.  A prompt's rows next to each other share the reading of their adapter.
     """
+    fast = _native_calls() if _fast is None else _fast
+    if fast:
+        made = fast.lora_add(base, x, a, b, ids, scales, out)
+        if made is not None:
+            return made
     device = _device_of("base", base)
     db, dx, da, dl = _describe("base", base, device), _describe("x", x, device), _describe("a", a, device), _describe("b", b, device)
     work = _workspace(_native.lib().tts_lora_add_workspace, device, dx, dl)
