@@ -137,7 +137,7 @@ tts_status tts_moe_route(const tts_tensor *logits, const tts_tensor *bias, int s
  * x [T, H] f16 or bf16, ids [T, k] i32, weights [T, k] f32, w_up [E, H, 2 I] with Wg its first I columns and Wu the others, w_down
  * [E, I, O], out [T, O] of x's type (it may be x: all of x is read before any of out is written).  Not `gated`: w_up [E, H, I], h = f(x[t] W[e]).
  * Weights are of x's type, or i8 with s_up [E, 2 I] and s_down [E, O] f32 that multiply their columns (NULL otherwise); each matrix
- * has stride 1 along its inputs or along its outputs.  H, I, O >= 8.  An id outside [0, E) contributes nothing; the same id
+ * has stride 1 along its inputs or along its outputs.  H, I, O >= 8, of i8 weights >= 16.  An id outside [0, E) contributes nothing; the same id
  * twice in a row contributes twice.  Sums, h and the weighted parts are held in 32 bits. */
 tts_status tts_moe_experts_workspace(const tts_tensor *x, const tts_tensor *ids, const tts_tensor *w_up, const tts_tensor *w_down, int gated,
                                      size_t *bytes);

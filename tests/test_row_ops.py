@@ -96,6 +96,7 @@ REFUSALS = [
     ("tts_moe_experts", experts_args, dict(w_down=tensor(BF16, 8, 96, 64)), N.TTS_INVALID, "w_down: dimension 1 is 96"),
     ("tts_moe_experts", experts_args, dict(w_down=tensor(I8, 8, 48, 64)), N.TTS_INVALID, "w_down is i8, not bf16"),
     ("tts_moe_experts", experts_args, dict(w_up=tensor(BF16, 8, 64, 8), w_down=tensor(BF16, 8, 4, 64)), N.TTS_UNSUPPORTED, "narrower than 8"),
+    ("tts_moe_experts", experts_args, dict(w_up=tensor(I8, 8, 64, 24), w_down=tensor(I8, 8, 12, 64)), N.TTS_UNSUPPORTED, "narrower than 16"),
     ("tts_moe_experts", experts_args, dict(s_up=tensor(F32, 8, 96)), N.TTS_INVALID, "scales belong to i8"),
     ("tts_moe_experts", experts_args, dict(w_up=tensor(I8, 8, 64, 96), w_down=tensor(I8, 8, 48, 64)), N.TTS_INVALID, "s_up is missing"),
     ("tts_moe_experts", experts_args, dict(activation=3), N.TTS_INVALID, "activation 3"),
@@ -308,10 +309,17 @@ def check_experts(a, activation="silu", out=None):
 @pytest.mark.gpu
 @pytest.mark.parametrize("order_up,order_down", [("in", "in"), ("out", "out"), ("in", "out"), ("out", "in")])
 @pytest.mark.parametrize("dtype,weights", [("bf16", None), ("fp16", None), ("bf16", "int8"), ("fp16", "int8")])
-@pytest.mark.parametrize("T,k,E,H,I,O,gated", [(1, 2, 8, 128, 64, 128, True), (3, 2, 4, 200, 72, 136, True), (17, 3, 5, 96, 160, 264, False), (5, 2, 6, 333, 75, 131, True), (2, 1, 3, 8, 8, 8, True),
+@pytest.mark.parametrize("T,k,E,H,I,O,gated", [(1, 2, 8, 128, 64, 128, True), (3, 2, 4, 200, 72, 136, True), (17, 3, 5, 96, 160, 264, False), (5, 2, 6, 333, 75, 131, True), (2, 1, 3, 16, 16, 16, True),
                                                (40, 4, 4, 70, 129, 65, False)])
 def test_experts(T, k, E, H, I, O, gated, dtype, weights, order_up, order_down):
     check_experts(make_experts(T, k, E, H, I, O, dtype, weights, order_up, order_down, gated, seed=T + I))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["in", "out"])
+def test_experts_of_the_narrowest_layer(order):
+    check_experts(make_experts(2, 1, 3, 8, 8, 8, "bf16", None, order, order, True))
+    check_experts(make_experts(3, 2, 3, 9, 11, 10, "fp16", None, order, order, False))
 
 
 @pytest.mark.gpu
@@ -319,6 +327,15 @@ def test_experts(T, k, E, H, I, O, gated, dtype, weights, order_up, order_down):
 @pytest.mark.parametrize("activation", ["silu", "gelu_tanh", "relu"])
 def test_experts_of_ordinary_sizes(T, k, E, H, I, O, activation):
     check_experts(make_experts(T, k, E, H, I, O, order_up="in", order_down="out"), activation)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("I,O", [(2072, 64), (24, 4100)])
+@pytest.mark.parametrize("dtype,weights,order", [("bf16", None, "in"), ("fp16", None, "out"), ("bf16", "int8", "in"), ("fp16", "int8", "out")])
+def test_experts_with_several_slabs_per_workgroup(I, O, dtype, weights, order):
+    a = make_experts(40, 2, 64, 40, I, O, dtype, weights, order, order)
+    a["ids"][:35, 0] = 7                    # and an expert whose rows take several turns
+    check_experts(a)
 
 
 @pytest.mark.gpu

@@ -58,9 +58,9 @@ __device__ __forceinline__ uint4 octet(const char *p) {
 }
 __device__ __forceinline__ uint4 octet_part(const char *p, int valid) {
   if (valid >= 8) return octet(p);
-  if (valid <= 0) return make_uint4(0, 0, 0, 0);
-  const Dwords<4> d = load_part<4, 2>(p, 2 * valid);
-  return make_uint4(d.d[0], d.d[1], d.d[2], d.d[3]);
+  u32 w[4] = {0, 0, 0, 0};
+  for (int i = 0; i < valid; i++) w[i >> 1] |= (u32)((const uint16_t *)p)[i] << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---- kernel 1: v[slice][t][r], 16 * MT rows and 16 * NB of the rank per workgroup; four wavefronts share the slice's steps of 32 inputs

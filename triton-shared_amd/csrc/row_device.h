@@ -42,12 +42,28 @@ __device__ __forceinline__ Dwords<DW> load_dwords(const char *p) {
   return v;
 }
 
-// the first `valid` bytes of them (in elements of ES bytes), zero behind
-template <int DW, int ES>
-__device__ __forceinline__ Dwords<DW> load_part(const char *p, int valid) {
-  Dwords<DW> v = {};
-  for (int i = 0; i < 4 * DW / ES; i++)
-    if (i * ES < valid) v.d[i * ES / 4] |= (ES == 2 ? (u32) * (const uint16_t *)(p + i * ES) : (u32) * (const uint8_t *)(p + i)) << (8 * (i * ES % 4));
+// the same for what is read once: it leaves the caches to what is read again
+template <int DW>
+__device__ __forceinline__ Dwords<DW> stream_dwords(const char *p) {
+  if constexpr (DW == 1) {
+    typedef u32 U1 __attribute__((aligned(1)));
+    return {__builtin_nontemporal_load((const U1 *)p)};
+  } else {
+    typedef u32 V __attribute__((ext_vector_type(DW)));
+    typedef V Unaligned __attribute__((aligned(1)));
+    return __builtin_bit_cast(Dwords<DW>, (V)__builtin_nontemporal_load((const Unaligned *)p));
+  }
+}
+
+// the first `valid` of 16 bytes, zeros behind: by a load that ends with them (the row they end has at least 16 bytes)
+__device__ __forceinline__ Dwords<4> load_part(const char *p, int valid) {
+  if (valid <= 0) return Dwords<4>{};
+  const int back = valid < 16 ? 16 - valid : 0;
+  Dwords<4> v = load_dwords<4>(p - back);
+  if (back & 8) v = {v.d[2], v.d[3], 0, 0};
+  if (back & 4) v = {v.d[1], v.d[2], v.d[3], 0};
+  const u32 next[4] = {v.d[1], v.d[2], v.d[3], 0};
+  each<0, 4>([&](auto ic) __attribute__((always_inline)) { v.d[ic.value] = __builtin_amdgcn_alignbyte(next[ic.value], v.d[ic.value], back & 3); });
   return v;
 }
 

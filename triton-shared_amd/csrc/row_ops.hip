@@ -126,7 +126,17 @@ tts_status guarded(const char *who, F &&f) {
   }
 }
 
-// what the sizes alone say, for the workspace and for the call
+ExpertMatrix matrix_of(const Arg &w) {
+  ExpertMatrix m = {};
+  m.w = w.t->ptr, m.w_expert = w.stride(0), m.w_k = w.stride(1), m.w_n = w.stride(2);
+  if (m.w_k != 1 && m.w_n != 1) invalid(w.name + ": neither its inputs (dimension 1) nor its outputs (dimension 2) have stride 1");
+  // the kernels' offsets within an expert are 32-bit: to a column's inputs, or to eight rows of them
+  const int64_t item = item_size(w.t->dtype), most = m.w_k == 1 ? w.size(2) * m.w_n + 64 : 32 * m.w_k + w.size(2);
+  if (most * item > 0xffffffffll) unsupported(w.name + ": strides of " + std::to_string(m.w_k) + " and " + std::to_string(m.w_n) + " reach past 4 GiB in one expert");
+  return m;
+}
+
+// what sizes, types and orders alone say, for the workspace and for the call
 ExpertsParams experts_sizes(const tts_tensor *x_, const tts_tensor *ids_, const tts_tensor *w_up_, const tts_tensor *w_down_, int gated) {
   Arg x(x_, "x"), ids(ids_, "ids"), w_up(w_up_, "w_up"), w_down(w_down_, "w_down");
   x.rank(2), ids.rank(2).type(TTS_I32).shape(0, x.size(0), "x").some(1), w_up.rank(3).shape(1, x.size(1), "x").some(0), w_down.rank(3).shape(0, w_up.size(0), "w_up");
@@ -138,21 +148,13 @@ ExpertsParams experts_sizes(const tts_tensor *x_, const tts_tensor *ids_, const 
   p.tokens = x.size(0), p.hidden = x.size(1), p.inner = gated ? w_up.size(2) / 2 : w_up.size(2), p.outputs = w_down.size(2);
   w_down.shape(1, p.inner, "w_up");
   p.experts = (int)w_up.size(0), p.gated = gated != 0, p.bf16 = x.t->dtype == TTS_BF16, p.int8 = w_up.t->dtype == TTS_I8;
-  if (p.hidden < 8 || p.inner < 8 || p.outputs < 8) unsupported("a layer narrower than 8 (" + std::to_string(p.hidden) + " x " + std::to_string(p.inner) + " x " + std::to_string(p.outputs) + ")");
+  const int least = p.int8 ? 16 : 8;  // 16 bytes of a row of weights
+  if (p.hidden < least || p.inner < least || p.outputs < least) unsupported("a layer narrower than " + std::to_string(least) + " (" + std::to_string(p.hidden) + " x " + std::to_string(p.inner) + " x " + std::to_string(p.outputs) + ")");
   if (ids.size(1) > EXPERTS_MAX_SLOTS || p.tokens * ids.size(1) > EXPERTS_MAX_SLOTS)
     unsupported(std::to_string(p.tokens) + " tokens of " + std::to_string(ids.size(1)) + " experts: more than " + std::to_string(EXPERTS_MAX_SLOTS) + " in all");
   p.top = (int)ids.size(1);
+  p.up = matrix_of(w_up), p.down = matrix_of(w_down);
   return p;
-}
-
-ExpertMatrix matrix_of(const Arg &w) {
-  ExpertMatrix m = {};
-  m.w = w.t->ptr, m.w_expert = w.stride(0), m.w_k = w.stride(1), m.w_n = w.stride(2);
-  if (m.w_k != 1 && m.w_n != 1) invalid(w.name + ": neither its inputs (dimension 1) nor its outputs (dimension 2) have stride 1");
-  // the kernels' offsets within an expert are 32-bit: to a column's inputs, or to eight rows of them
-  const int64_t item = item_size(w.t->dtype), most = m.w_k == 1 ? w.size(2) * m.w_n + 64 : 32 * m.w_k + w.size(2);
-  if (most * item > 0xffffffffll) unsupported(w.name + ": strides of " + std::to_string(m.w_k) + " and " + std::to_string(m.w_n) + " reach past 4 GiB in one expert");
-  return m;
 }
 
 LoraParams lora_sizes(const tts_tensor *x_, const tts_tensor *b_) {
@@ -222,7 +224,6 @@ tts_status tts_moe_experts(const tts_tensor *x_, const tts_tensor *ids_, const t
     weights.rank(2).type(TTS_F32).shape(0, p.tokens, "x").shape(1, p.top, "ids").neighbours();
     out.rank(2).type(x.t->dtype).shape(0, p.tokens, "x").shape(1, p.outputs, "w_down").neighbours().distinct();
     x.present(), ids.present(), weights.present(), w_up.present(), w_down.present(), out.present();
-    p.up = matrix_of(w_up), p.down = matrix_of(w_down);
     if (p.int8) {
       Arg s_up(s_up_, "s_up"), s_down(s_down_, "s_down");
       s_up.rank(2).type(TTS_F32).shape(0, p.experts, "w_up").shape(1, w_up.size(2), "w_up").neighbours().present();
