@@ -65,7 +65,9 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteParams p) {
     }
   }
   unsigned taken = 0;
-  float total = 0.f;
+  float total = 0.f, held[ROUTE_MAX_TOP / G];  // lane i holds choices i, i + G, ...
+  int chosen[ROUTE_MAX_TOP / G];
+  for (int h = 0; h < ROUTE_MAX_TOP / G; h++) held[h] = 0.f, chosen[h] = -1;
   for (int n = 0; n < p.top; n++) {
     C best = -INFINITY;
     int at = -1;
@@ -77,24 +79,30 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteParams p) {
     const int expert = over_lanes<G>(mine, [](int a, int b) { return a < b ? a : b; });
     const bool any = expert != INT_MAX;
     if (any && expert == mine) taken |= 1u << at;
-    // the chosen one's score, from its logit
-    const float z = __shfl(logit, any ? expert % G : 0, G);
+    const float z = __shfl(logit, any ? expert % G : 0, G);  // the chosen one's logit
+    for (int h = 0; h < ROUTE_MAX_TOP / G; h++)
+      if (n == h * G + lane) held[h] = z, chosen[h] = any ? expert : -1;
+  }
+  // the scores of the chosen ones, all at once
+  for (int h = 0; h < ROUTE_MAX_TOP / G; h++) {
+    const float z = held[h];
     float s = 0.f;
-    if (any) s = p.sigmoid ? (float)(1.0 / (1.0 + exp(-(double)z))) : expf(z - most);
-    if (any && !p.sigmoid && !p.renormalize) s = (float)((C)s / sum);
-    if (nan && any) s = NAN;
+    if (chosen[h] >= 0) {
+      s = p.sigmoid ? (float)(1.0 / (1.0 + exp(-(double)z))) : expf(z - most);
+      if (!p.sigmoid && !p.renormalize) s = (float)((C)s / sum);
+      if (nan) s = NAN;
+    }
+    held[h] = s;
     total += s;
-    if (live && lane == 0) {
-      p.ids[token * p.ld_ids + n] = any ? expert : -1;
-      p.weights[token * p.ld_weights + n] = s;
+  }
+  total = over_lanes<G>(total, [](float a, float b) { return a + b; });
+  for (int h = 0; h < ROUTE_MAX_TOP / G; h++) {
+    const int n = h * G + lane;
+    if (live && n < p.top) {
+      p.ids[token * p.ld_ids + n] = chosen[h];
+      p.weights[token * p.ld_weights + n] = held[h] == 0.f ? 0.f : held[h] / (p.renormalize ? total : 1.f) * p.scale;
     }
   }
-  // (the same lane wrote them)
-  if (live && lane == 0)
-    for (int n = 0; n < p.top; n++) {
-      float *w = p.weights + token * p.ld_weights + n;
-      *w = *w == 0.f ? 0.f : *w / (p.renormalize ? total : 1.f) * p.scale;
-    }
 }
 
 template <class T, class C>

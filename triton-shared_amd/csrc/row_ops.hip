@@ -165,7 +165,7 @@ LoraParams lora_sizes(const tts_tensor *x_, const tts_tensor *b_) {
   LoraParams p = {};
   p.tokens = x.size(0), p.inputs = x.size(1), p.adapters = (int)b.size(0), p.outputs = b.size(1);
   if (b.size(2) > LORA_MAX_RANK) unsupported("b: a rank of " + std::to_string(b.size(2)) + ", more than " + std::to_string(LORA_MAX_RANK));
-  if (p.tokens > 64 * 65535) unsupported("x: " + std::to_string(p.tokens) + " rows");
+  if (p.tokens > 32 * 65535) unsupported("x: " + std::to_string(p.tokens) + " rows");
   p.rank = (int)b.size(2), p.bf16 = x.t->dtype == TTS_BF16;
   return p;
 }
@@ -261,6 +261,7 @@ tts_status tts_lora_add(const tts_tensor *base_, const tts_tensor *x_, const tts
     out.rank(2).type(x.t->dtype).shape(0, p.tokens, "x").shape(1, p.outputs, "b").neighbours().distinct();
     a.rank(3).type(x.t->dtype).shape(0, p.adapters, "b").shape(1, p.rank, "b").shape(2, p.inputs, "x").neighbours();
     ids.rank(1).type(TTS_I32).shape(0, p.tokens, "x");
+    if (2 * (a.size(1) * a.stride(1) + 64) > 0xffffffffll) unsupported("a: rows " + std::to_string(a.stride(1)) + " apart reach past 4 GiB in one adapter");
     base.present(), x.present(), a.present(), b.present(), ids.present(), out.present();
     if (scales_) {
       Arg scales(scales_, "scales");
