@@ -233,6 +233,27 @@ def test_route_ties_masks_and_nan(experts, scoring, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [40, 250, 600])
+def test_route_scores_that_32_bits_cannot_tell_apart(scoring, experts):
+    # biases that bring the scores to the same value but for some 2^-30 of it, rising with the expert in half of the rows' experts
+    logits = gpu(1, experts, seed=11, scale=1.5)
+    l = logits[0].double()
+    s = torch.sigmoid(l) if scoring == "sigmoid" else torch.softmax(l, 0)
+    bias = (1.5 - s).float()                # rounded: s + bias is 1.5 but for half a step of it
+    check_route(logits, 9, scoring, bias)
+    many = logits.repeat(70, 1)
+    many[::3, 5] += 0.75                    # some rows have one that stands out
+    check_route(many, 9, scoring, bias)
+    check_route(many, 9, scoring, torch.full_like(bias, 1e6))
+    bias[3] = float("inf")                  # always chosen
+    bias[4], bias[6] = float("-inf"), float("nan")
+    many[:, 7] = float("-inf")
+    check_route(many, 1, scoring, bias)
+    check_route(many, 4, scoring, bias)
+
+
+@pytest.mark.gpu
 def test_route_of_columns_of_a_wider_buffer():
     wide = gpu(21, 300, seed=8, dtype="bf16")
     check_route(wide[:, 7:107], 5)
@@ -357,7 +378,7 @@ def test_experts_ids_outside_repeated_and_one_for_all(dtype):
 
 @pytest.mark.gpu
 def test_experts_with_more_experts_than_slots_and_back():
-    for T, E in ((3, 64), (3, 4), (1, 3), (2, 2)):
+    for T, E in ((3, 64), (3, 4), (1, 3), (2, 2), (40, 100), (50, 101)):  # (with more than 64 slots: found by all wavefronts together)
         a = make_experts(T, 2, E, 64, 64, 64)
         a["ids"][0, 1] = a["ids"][T - 1, 0]  # one expert in two rows
         check_experts(a)
