@@ -58,12 +58,14 @@ __device__ __forceinline__ uint4 octet(const char *p) {
   return v;
 }
 // How rows end.  (The checks at every load would be most of a kernel's code, and a launch for few rows waits for its code.)
-enum Ends { EVEN = 0,   // with a whole octet
+enum Ends { EXACT = 3,  // with a whole step of 64
+            EVEN = 0,   // with a whole octet
             LONG = 1,   // anywhere, at least eight elements from their beginning: the last octet's load is moved back to end with the row
             SHORT = 2 };
 template <int ENDS>
 __device__ __forceinline__ uint4 octet_part(const char *p, int valid) {
-  if constexpr (ENDS == EVEN) {
+  if constexpr (ENDS == EXACT) return octet(p);
+  else if constexpr (ENDS == EVEN) {
     uint4 v = make_uint4(0, 0, 0, 0);
     if (valid > 0) v = octet(p);
     return v;
@@ -87,9 +89,9 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p, Shape sh
   const int64_t row0 = (int64_t)blockIdx.x * (16 * MT);
   const int r0 = blockIdx.z * (16 * NB);
   const int my_id = lane < 16 * MT ? row_id(p, row0 + lane) : -1;
-  const int K = (int)p.inputs, whole = K / 64, steps = (K + 63) / 64;
+  const int K = (int)p.inputs, steps = (K + 63) / 64;
   const int share = (int)blockIdx.y * 4 + wave, shares = sh.slices * 4;
-  const int begin = (int)((int64_t)share * steps / shares), end_all = (int)((int64_t)(share + 1) * steps / shares), end = min(end_all, whole);
+  const int begin = (int)((int64_t)share * steps / shares), end = (int)((int64_t)(share + 1) * steps / shares);
   const char *x[MT];
   each<0, MT>([&](auto mc) __attribute__((always_inline)) {
     const int64_t row = row0 + 16 * mc.value + c;
@@ -106,25 +108,17 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p, Shape sh
   each<0, MT * NB>([&](auto ic) __attribute__((always_inline)) { acc[ic.value / NB][ic.value % NB] = (f32x4){0.f, 0.f, 0.f, 0.f}; });
   // (halves: k 8 g .. and 32 + 8 g ..)
   auto load_x = [&](int s, uint4 (&xs)[2][MT]) __attribute__((always_inline)) {
-    each<0, 2 * MT>([&](auto nc) __attribute__((always_inline)) { xs[nc.value % 2][nc.value / 2] = octet(x[nc.value / 2] + 128 * (int64_t)s + 64 * (nc.value % 2)); });
+    each<0, 2 * MT>([&](auto nc) __attribute__((always_inline)) { xs[nc.value % 2][nc.value / 2] = octet_part<ENDS>(x[nc.value / 2] + 128 * (int64_t)s + 64 * (nc.value % 2), K - 64 * s - 32 * (nc.value % 2) - 8 * g); });
   };
   auto load_a = [&](const char *a, int s, uint4 (&as)[2][NB]) __attribute__((always_inline)) {
     const char *at = a + 128 * (int64_t)s;
-    each<0, 2 * NB>([&](auto nc) __attribute__((always_inline)) { as[nc.value % 2][nc.value / 2] = octet(at + a_off[nc.value / 2] + 64 * (nc.value % 2)); });
+    each<0, 2 * NB>([&](auto nc) __attribute__((always_inline)) { as[nc.value % 2][nc.value / 2] = octet_part<ENDS>(at + a_off[nc.value / 2] + 64 * (nc.value % 2), K - 64 * s - 32 * (nc.value % 2) - 8 * g); });
   };
   auto add = [&](const uint4 (&xs)[2][MT], const uint4 (&as)[2][NB]) __attribute__((always_inline)) {
     each<0, 2 * MT * NB>([&](auto nc) __attribute__((always_inline)) {
       constexpr int h = nc.value / (MT * NB), m = nc.value / NB % MT, i = nc.value % NB;
       acc[m][i] = mfma16<BF16>(xs[h][m], as[h][i], acc[m][i]);
     });
-  };
-  uint4 xp[2][MT], ap[2][NB];  // the part step
-  const int valid = K - 64 * whole - 8 * g;
-  auto load_part_x = [&]() __attribute__((always_inline)) {
-    each<0, 2 * MT>([&](auto nc) __attribute__((always_inline)) { xp[nc.value % 2][nc.value / 2] = octet_part<ENDS>(x[nc.value / 2] + 128 * (int64_t)whole + 64 * (nc.value % 2), valid - 32 * (nc.value % 2)); });
-  };
-  auto load_part_a = [&](const char *a) __attribute__((always_inline)) {
-    each<0, 2 * NB>([&](auto nc) __attribute__((always_inline)) { ap[nc.value % 2][nc.value / 2] = octet_part<ENDS>(a + a_off[nc.value / 2] + 128 * (int64_t)whole + 64 * (nc.value % 2), valid - 32 * (nc.value % 2)); });
   };
   if (n == 1) {
     constexpr int U = MT + NB >= 4 ? 2 : 4;
@@ -149,11 +143,6 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p, Shape sh
       each<0, U>([&](auto uc) __attribute__((always_inline)) {
         if (s + uc.value < end) add(xs[uc.value], as[uc.value]);
       });
-    }
-    if (end_all > whole) {
-      load_part_x();
-      load_part_a(a);
-      add(xp, ap);
     }
   } else {
     int of_sum[MT][4];  // the adapters of the rows whose sums the lane holds
@@ -190,13 +179,6 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p, Shape sh
           }
           fetch(as[uc.value]);
         });
-    }
-    if (end_all > whole) {
-      load_part_x();
-      for (int d = 0; d < n; d++) {
-        load_part_a(weights_of(adapter(d)));
-        add_own(xp, ap, adapter(d));
-      }
     }
   }
   each<0, MT>([&](auto mc) __attribute__((always_inline)) {
@@ -271,7 +253,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p, Shape sh
     __syncthreads();
   };
   // a tile's loads of base, and of the first adapters: on their way before v is staged, and before the tile before is stored
-  constexpr int U = MT > 1 ? 2 : 4;
+  constexpr int U = MT > 1 || ENDS != EVEN ? 2 : 4;
   const bool once = p.rank <= CHUNK;
   uint4 e[MT][2], ring[U][4];
   int64_t b_off[4], col = 0;
@@ -409,7 +391,8 @@ hipError_t launch_rows(const LoraParams &p, const Shape &sh, hipStream_t s) {
     lora_expand_kernel<BF16, decltype(ends)::value, MT2>
         <<<dim3((unsigned)(((p.outputs + 255) / 256 + sh.columns_each - 1) / sh.columns_each), sh.row_tiles_of_2), 256, 0, s>>>(p, sh, v);
   };
-  if (p.inputs % 8 == 0) shrink_in(Int<EVEN>{});
+  if (p.inputs % 64 == 0) shrink_in(Int<EXACT>{});
+  else if (p.inputs % 8 == 0) shrink_in(Int<EVEN>{});
   else if (p.inputs > 8) shrink_in(Int<LONG>{});
   else shrink_in(Int<SHORT>{});
   const hipError_t e = hipGetLastError();
