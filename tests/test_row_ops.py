@@ -97,6 +97,7 @@ REFUSALS = [
     ("tts_moe_experts", experts_args, dict(w_down=tensor(I8, 8, 48, 64)), N.TTS_INVALID, "w_down is i8, not bf16"),
     ("tts_moe_experts", experts_args, dict(w_up=tensor(BF16, 8, 64, 8), w_down=tensor(BF16, 8, 4, 64)), N.TTS_UNSUPPORTED, "narrower than 8"),
     ("tts_moe_experts", experts_args, dict(w_up=tensor(I8, 8, 64, 24), w_down=tensor(I8, 8, 12, 64)), N.TTS_UNSUPPORTED, "narrower than 16"),
+    ("tts_moe_experts", experts_args, dict(w_up=tensor(BF16, 8, 64, 1 << 26, stride=(64, 1, 1)), w_down=tensor(BF16, 8, 1 << 25, 64)), N.TTS_UNSUPPORTED, "wider than 16777216"),
     ("tts_moe_experts", experts_args, dict(s_up=tensor(F32, 8, 96)), N.TTS_INVALID, "scales belong to i8"),
     ("tts_moe_experts", experts_args, dict(w_up=tensor(I8, 8, 64, 96), w_down=tensor(I8, 8, 48, 64)), N.TTS_INVALID, "s_up is missing"),
     ("tts_moe_experts", experts_args, dict(activation=3), N.TTS_INVALID, "activation 3"),

@@ -610,8 +610,17 @@ int row_blocks(const ExpertsParams &p) {
 
 constexpr int WAVES = 4;
 
-template <bool BF16, bool I8>
-hipError_t launch_typed(const ExpertsParams &p, hipStream_t s) {
+}  // namespace
+
+// The kernels of one type of activations and weights, for up to 32 rows of an expert at once or for more (MANY).  This file is compiled once for
+// each of the eight (TTS_EXPERTS_PART: bit 0 bf16, bit 1 int8, bit 2 MANY), side by side, and once for what picks among them.
+template <bool BF16, bool I8, bool MANY>
+hipError_t launch_experts_as(const ExpertsParams &p, hipStream_t s);
+
+#ifdef TTS_EXPERTS_PART
+
+template <bool BF16, bool I8, bool MANY>
+hipError_t launch_experts_as(const ExpertsParams &p, hipStream_t s) {
   const Layout l = layout_of(p, h_cols(p));
   const int groups = groups_of(p), by_slot = groups < p.experts;
   const int nb_up = up_blocks(p), nb_down = blocks_of<I8>(p.down, p.outputs, groups, 16);
@@ -638,20 +647,29 @@ hipError_t launch_typed(const ExpertsParams &p, hipStream_t s) {
     if (p.down.w_k != 1) return nb_down == (I8 ? 16 : 8) ? down(Int<0>{}, mt, Int<I8 ? 16 : 8>{}) : down(Int<0>{}, mt, Int<I8 ? 8 : 4>{});
     return nb_down == 8 ? down(Int<1>{}, mt, Int<8>{}) : down(Int<1>{}, mt, Int<4>{});
   };
-  const int rows = row_blocks(p);
-  const hipError_t e = rows == 1 ? with_rows(Int<1>{}) : rows == 2 ? with_rows(Int<2>{}) : with_rows(Int<4>{});
+  hipError_t e;
+  if constexpr (MANY) e = with_rows(Int<4>{});
+  else e = row_blocks(p) == 1 ? with_rows(Int<1>{}) : with_rows(Int<2>{});
   if (e != hipSuccess) return e;
   experts_sum_kernel<BF16><<<dim3((unsigned)((p.outputs + 255) / 256), (unsigned)p.tokens), 256, 0, s>>>(p, l.partial);
   return hipGetLastError();
 }
 
-}  // namespace
+template hipError_t launch_experts_as<(TTS_EXPERTS_PART & 1) != 0, (TTS_EXPERTS_PART & 2) != 0, (TTS_EXPERTS_PART & 4) != 0>(const ExpertsParams &, hipStream_t);
+
+#else
 
 size_t experts_workspace_bytes(const ExpertsParams &p) { return layout_of(p, h_cols(p)).bytes; }
 
 hipError_t launch_experts(const ExpertsParams &p, hipStream_t s) {
-  if (p.bf16) return p.int8 ? launch_typed<true, true>(p, s) : launch_typed<true, false>(p, s);
-  return p.int8 ? launch_typed<false, true>(p, s) : launch_typed<false, false>(p, s);
+  auto of = [&](auto many) {
+    constexpr bool MANY = decltype(many)::value != 0;
+    if (p.bf16) return p.int8 ? launch_experts_as<true, true, MANY>(p, s) : launch_experts_as<true, false, MANY>(p, s);
+    return p.int8 ? launch_experts_as<false, true, MANY>(p, s) : launch_experts_as<false, false, MANY>(p, s);
+  };
+  return row_blocks(p) > 2 ? of(Int<1>{}) : of(Int<0>{});
 }
+
+#endif
 
 }  // namespace tts

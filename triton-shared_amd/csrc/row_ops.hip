@@ -31,6 +31,8 @@ const char *type_name(int dtype) {
 
 constexpr int64_t MOST_SIZE = (int64_t)1 << 30;  // of a dimension: sums of two fit 32 bits
 
+constexpr int64_t MOST_WIDTH = (int64_t)1 << 24;  // of a layer: its tiles times its slots fit a grid
+
 // one argument of a call, by its name
 struct Arg {
   const tts_tensor *t;
@@ -150,6 +152,7 @@ ExpertsParams experts_sizes(const tts_tensor *x_, const tts_tensor *ids_, const 
   p.experts = (int)w_up.size(0), p.gated = gated != 0, p.bf16 = x.t->dtype == TTS_BF16, p.int8 = w_up.t->dtype == TTS_I8;
   const int least = p.int8 ? 16 : 8;  // 16 bytes of a row of weights
   if (p.hidden < least || p.inner < least || p.outputs < least) unsupported("a layer narrower than " + std::to_string(least) + " (" + std::to_string(p.hidden) + " x " + std::to_string(p.inner) + " x " + std::to_string(p.outputs) + ")");
+  if (p.inner > MOST_WIDTH || p.outputs > MOST_WIDTH) unsupported("a layer wider than " + std::to_string(MOST_WIDTH) + " (" + std::to_string(p.inner) + ", " + std::to_string(p.outputs) + ")");
   if (ids.size(1) > EXPERTS_MAX_SLOTS || p.tokens * ids.size(1) > EXPERTS_MAX_SLOTS)
     unsupported(std::to_string(p.tokens) + " tokens of " + std::to_string(ids.size(1)) + " experts: more than " + std::to_string(EXPERTS_MAX_SLOTS) + " in all");
   p.top = (int)ids.size(1);
