@@ -6,7 +6,9 @@
 // multiplied by zero: an infinity in one request's adapter stays with that request.)
 // v is summed and kept in 32 bits, in slices of the inputs that kernel 2 adds as it reads them; it enters the second product as
 // two 16-bit parts (row_device.h).
-// What has to move is x, base and out once and the adapters: memory or, for few rows, the launches.
+// What has to move is x, base and out once and the adapters.  What bounds it: few rows, the launches and chains of loads (one row of 4096 x 4096, rank
+// 16: 4 + 7 us; 64 rows with an adapter each, 4096 x 8192: 10 + 15 us, up to 16 adapters in turn per tile, eight loads ahead); prompts, the chain of
+// load, product and store in two workgroups per CU (8192 rows, rank 64: 37 us for 67 MB of x, 60 us for 134 MB of base and out, 2.2 TB/s).
 #include <algorithm>
 #include <cmath>
 
