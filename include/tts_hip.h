@@ -126,9 +126,9 @@ typedef enum tts_activation { TTS_SILU = 0, TTS_GELU_TANH = 1, TTS_RELU = 2 } tt
  * weights [T, k] f32 (k <= 64) written; rows any distance apart, elements of a row neighbours.  With s = softmax or sigmoid of a
  * row's logits, ids are the k experts of the largest s + bias (without a bias: of the largest logits, which is the same order where
  * neither score has run into 0 or 1), in descending order, ties to the lowest expert, and weights are scale * s, divided by
- * the sum of the chosen s if `renormalize` (0 where s is 0).  Logits of -inf are
- * not chosen, nor is an s + bias that is -inf or NaN; where fewer than k are left, ids are -1 and weights 0.  A row that
- * holds a NaN has weights of NaN. */
+ * the sum of the chosen s if `renormalize`: as the formula says also where all chosen s are too small for 32 bits, but 0 where s is
+ * under e^-745 (a mask of the type's lowest value).  Logits of -inf are not chosen, nor is an s + bias that is
+ * -inf or NaN; where fewer than k are left, ids are -1 and weights 0.  A row that holds a NaN has weights of NaN. */
 tts_status tts_moe_route(const tts_tensor *logits, const tts_tensor *bias, int scoring, int renormalize, double scale,
                          const tts_tensor *ids, const tts_tensor *weights, void *stream);
 

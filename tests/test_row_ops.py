@@ -255,6 +255,39 @@ def test_route_scores_that_32_bits_cannot_tell_apart(scoring, experts):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("experts", [24, 200, 700])
+@pytest.mark.parametrize("bias", [False, True])
+def test_route_sigmoids_below_32_bits_keep_their_ratio(bias, experts, dtype):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(experts)
+    logits = torch.empty(9, experts, device="cuda").uniform_(-200.0, -90.0, generator=g)
+    for i, l in enumerate((-20.0, -86.0, -100.0, -103.0, -110.0, -600.0)):  # two of them, one apart, and others far below
+        logits[i] = -690.0
+        logits[i, 3], logits[i, 11] = l, l - 1.0
+    logits[6, 4] = 2.0                              # one that is not small
+    logits[7] = torch.finfo(TYPES[dtype]).min       # a mask that leaves nothing: no weights
+    logits[8] = 0.25 - (torch.arange(experts, device="cuda") % 7).float()
+    logits = logits.to(TYPES[dtype])
+    add = (torch.arange(experts, device="cuda") % 5 == 3).float() if bias else None  # (3 among them, and others of lower scores)
+    check_route(logits, 2, "sigmoid", add)
+    check_route(logits, 6, "sigmoid", add, scale=2.5)
+    check_route(logits, 6, "sigmoid", add, renormalize=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts", [24, 200, 700])
+def test_route_a_bias_that_chooses_far_below_the_largest_logit(experts):
+    logits = gpu(5, experts, seed=experts, scale=2.0)
+    logits[0, 1] = 95.0
+    logits[1, 1], logits[2, 1] = 120.0, 400.0
+    logits[3, 1] = 1e30                             # ... so far that nothing of the others is left
+    add = torch.where(torch.arange(experts, device="cuda") % 2 == 0, 4.0, 0.0)
+    check_route(logits, 8, "softmax", add)
+    check_route(logits, 8, "softmax", add, renormalize=False)
+
+
+@pytest.mark.gpu
 def test_route_of_columns_of_a_wider_buffer():
     wide = gpu(21, 300, seed=8, dtype="bf16")
     check_route(wide[:, 7:107], 5)

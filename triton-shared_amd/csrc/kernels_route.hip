@@ -85,6 +85,9 @@ __device__ __forceinline__ float sigmoid(float l) {
   return (l < 0.f ? x : 1.f) / (1.f + x);
 }
 
+// The logarithm under which a score is 0 (64 bits hold none there): experts that a mask of the type's lowest value leaves have no weight.
+constexpr float NO_SCORE = -745.f;
+
 // G lanes per token; lane i of them holds experts i, i + G, ... (N of them).  Which expert is chosen shows whole, so where scores get a bias
 // the choice is that of c in 64 bits: 32 bits decide it unless two that matter are near each other, which is seldom (a token in a thousand of
 // the one measured); then the candidates' c is computed in 64 bits and the choice made again.
@@ -160,19 +163,36 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteParams p) {
   } else
     choose<float, G, N>(l, lane, p.top, chosen, 0.f, nullptr, nullptr);
   // the scores of the chosen ones, all at once
-  float total = 0.f;
-  for (int h = 0; h < ROUTE_MAX_TOP / G; h++) {
-    float s = 0.f;
-    if (chosen[h] >= 0) {
-      const float z = widen<T>(row[chosen[h]]);
-      s = p.sigmoid ? sigmoid(z) : expf(z - most);
-      if (!p.sigmoid && !p.renormalize) s /= sum;
-      if (nan) s = NAN;
+  float z[ROUTE_MAX_TOP / G], total = 0.f;
+  for (int h = 0; h < ROUTE_MAX_TOP / G; h++) z[h] = chosen[h] >= 0 ? widen<T>(row[chosen[h]]) : -INFINITY;
+  auto hold = [&](auto score) __attribute__((always_inline)) {
+    total = 0.f;
+    for (int h = 0; h < ROUTE_MAX_TOP / G; h++) {
+      float s = 0.f;
+      if (chosen[h] >= 0) s = nan ? NAN : score(z[h]);
+      held[h] = s;
+      total += s;
     }
-    held[h] = s;
-    total += s;
+    total = over_lanes<G>(total, add);
+  };
+  hold([&](float z) __attribute__((always_inline)) {
+    if (p.sigmoid) return sigmoid(z);
+    const float s = expf(z - most);
+    return p.renormalize ? s : s / sum;
+  });
+  if (p.renormalize && total < 0.5f) {
+    // Some may be below what 32 bits hold, and not small in the sum of them: again without the factor that takes them all there, which
+    // divides out.  exp(z) is exp(z - largest), and where all are negative sigmoid(z) = exp(z) / (1 + exp(z)) is exp(z - largest) / (1 + exp(z)).
+    // (In every row instead: 21.8 us of the 16384 tokens below instead of 21.6.)
+    float largest = z[0];
+    for (int h = 1; h < ROUTE_MAX_TOP / G; h++) largest = fmaxf(largest, z[h]);
+    largest = over_lanes<G>(largest, [](float a, float b) { return fmaxf(a, b); });
+    hold([&](float z) __attribute__((always_inline)) {
+      if (z - (p.sigmoid ? 0.f : most) < NO_SCORE) return 0.f;
+      if (p.sigmoid) return largest < 0.f ? expf(z - largest) / (1.f + expf(z)) : sigmoid(z);
+      return expf(z - largest);
+    });
   }
-  total = over_lanes<G>(total, add);
   for (int h = 0; h < ROUTE_MAX_TOP / G; h++) {
     const int n = h * G + lane;
     if (live && n < p.top) {
