@@ -128,7 +128,8 @@ typedef enum tts_activation { TTS_SILU = 0, TTS_GELU_TANH = 1, TTS_RELU = 2 } tt
  * neither score has run into 0 or 1), in descending order, ties to the lowest expert, and weights are scale * s, divided by
  * the sum of the chosen s if `renormalize`: as the formula says also where all chosen s are too small for 32 bits, but 0 where s is
  * under e^-745 (a mask of the type's lowest value).  Logits of -inf are not chosen, nor is an s + bias that is
- * -inf or NaN; where fewer than k are left, ids are -1 and weights 0.  A row that holds a NaN has weights of NaN. */
+ * -inf or NaN; where fewer than k are left, ids are -1 and weights 0.  A row that holds a NaN has weights of NaN,
+ * and so has the softmax of one that holds +inf (its ids are those of the limit of ever larger logits). */
 tts_status tts_moe_route(const tts_tensor *logits, const tts_tensor *bias, int scoring, int renormalize, double scale,
                          const tts_tensor *ids, const tts_tensor *weights, void *stream);
 

@@ -288,6 +288,42 @@ def test_route_a_bias_that_chooses_far_below_the_largest_logit(experts):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("experts", [24, 200, 700])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias,renormalize", [(False, True), (False, False), (True, True), (True, False)])
+def test_route_infinite_logits(bias, renormalize, scoring, experts, dtype):
+    # softmax of a row with one is NaN: NaN weights, of the experts that the limit of ever larger logits picks
+    logits = gpu(7, experts, seed=experts + 1, scale=2.0, dtype=dtype)
+    inf = float("inf")
+    logits[0, 5] = inf
+    logits[1, 5], logits[1, 20], logits[1, 7] = inf, inf, -inf
+    logits[2] = inf
+    logits[3], logits[3, 9] = -inf, inf
+    logits[4, 6], logits[4, 9], logits[4, 2] = torch.finfo(TYPES[dtype]).max, inf, torch.finfo(TYPES[dtype]).min
+    logits[5, 6], logits[5, 9] = float("nan"), inf
+    add = (torch.arange(experts, device="cuda") % 4).float() * 0.25 if bias else None
+    ids, weights = (t.cpu().numpy() for t in ops.moe_route(logits, 4, scoring=scoring, bias=add, renormalize=renormalize))
+    for t, l in enumerate(logits.double().cpu().numpy()):
+        if scoring == "sigmoid":
+            with np.errstate(all="ignore"):
+                s = 1.0 / (1.0 + np.exp(-l))
+        elif np.isposinf(l).any():
+            s = np.isposinf(l) / np.isposinf(l).sum()
+        else:
+            s = np.exp(l - l.max()) / np.exp(l - l.max()).sum()
+        c = s + add.double().cpu().numpy() if bias else l
+        chosen = sorted((i for i in range(experts) if l[i] > -np.inf), key=lambda i: (-c[i], i))[:4]
+        assert list(ids[t]) == chosen + [-1] * (4 - len(chosen)), f"row {t}"
+        if np.isnan(l).any() or (scoring == "softmax" and np.isposinf(l).any()):
+            assert np.isnan(weights[t, :len(chosen)]).all() and not weights[t, len(chosen):].any(), f"row {t}"
+        else:
+            w = s[chosen] / (s[chosen].sum() if renormalize else 1.0)
+            # arguments of an exponential up to 13 (or one past 88, whose exponential is below 2^-126), and as in check_route
+            assert np.all(np.abs(weights[t, :len(chosen)] - w) <= U * (2 * 13 + 64 + 12) * w + 2.0 ** -126), f"row {t}"
+
+
+@pytest.mark.gpu
 def test_route_of_columns_of_a_wider_buffer():
     wide = gpu(21, 300, seed=8, dtype="bf16")
     check_route(wide[:, 7:107], 5)

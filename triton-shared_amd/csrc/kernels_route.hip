@@ -2,7 +2,8 @@
 //   s = softmax(l) or sigmoid(l);  c = s + bias, or l itself without a bias (the same order, and no two logits that differ
 //   become equal);  the `top` largest c, ties to the lowest expert;  weight = scale * s / (the sum of the chosen s).
 // A logit of -inf (a masked expert), a c of -inf and a NaN are never chosen; where fewer than `top` are left the rest of the row is expert -1
-// of weight 0.  A row that holds a NaN has NaN for its chosen experts' weights, as the formula gives.
+// of weight 0.  A row that holds a NaN has NaN for its chosen experts' weights, as the formula gives, and so has the softmax of one that holds +inf.
+#include <cfloat>
 #include <cmath>
 
 #include "kernels.h"
@@ -114,6 +115,13 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteParams p) {
   }
   most = over_lanes<G>(most, [](float a, float b) { return fmaxf(a, b); });
   nan = over_lanes<G>((int)nan, [](int a, int b) { return a | b; });
+  if (!p.sigmoid && most == INFINITY) {  // the softmax is NaN, and what is chosen is told by its limit: infinite logits share it, nothing is left for others
+    nan = true;
+    if constexpr (BIAS) {
+      for (int j = 0; j < N; j++) l[j] = l[j] == INFINITY ? 0.f : l[j] > -INFINITY ? -FLT_MAX : l[j];
+      most = 0.f;
+    }
+  }
   int chosen[ROUTE_MAX_TOP / G];
   float held[ROUTE_MAX_TOP / G], sum = 0.f;
   const auto add = [](auto a, auto b) { return a + b; };

@@ -92,7 +92,8 @@ def moe_route(logits, k, scoring="softmax", bias=None, renormalize=True, scale=1
     With s the softmax or the sigmoid of a row, ids are the experts of the k largest s + bias (without a bias: the k largest logits),
     largest first, ties to the lowest expert; weights are scale * s, over the sum of the chosen s if `renormalize` (right also
     where 32 bits hold none of them; under e^-745 s counts as 0).  Logits of -inf are never chosen: where fewer
-    than k others are left, ids are -1 and weights 0.  A row that holds a NaN gets weights of NaN.
+    than k others are left, ids are -1 and weights 0.  A row that holds a NaN gets weights of NaN, as does the softmax of
+    one that holds +inf.
     """
     fast = _native_calls() if _fast is None else _fast
     if fast:
