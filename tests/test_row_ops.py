@@ -333,6 +333,20 @@ def test_route_of_columns_of_a_wider_buffer():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.gpu
+def test_route_of_more_tokens_than_one_grid():
+    # 16 lanes a token: 2^28 of them are 2^32 lanes, more than a launch may have
+    tokens = 2 ** 28 + 19
+    logits = torch.zeros(tokens, 1, dtype=torch.bfloat16, device="cuda")
+    logits[-1] = float("-inf")
+    logits[2 ** 27 + 3] = float("nan")      # (a NaN is never chosen)
+    ids, weights = ops.moe_route(logits, 1)
+    for t in (2 ** 27 + 3, -1):
+        assert int(ids[t]) == -1 and float(weights[t]) == 0.0
+        ids[t], weights[t] = 0, 1.0
+    assert not ids.any() and bool((weights == 1.0).all())
+
+
 # ---------------------------------------------------------------------------------------------------------------- the experts
 def activation_exact(name, v):
     if name == "silu":

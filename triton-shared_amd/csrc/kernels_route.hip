@@ -3,6 +3,7 @@
 //   become equal);  the `top` largest c, ties to the lowest expert;  weight = scale * s / (the sum of the chosen s).
 // A logit of -inf (a masked expert), a c of -inf and a NaN are never chosen; where fewer than `top` are left the rest of the row is expert -1
 // of weight 0.  A row that holds a NaN has NaN for its chosen experts' weights, as the formula gives, and so has the softmax of one that holds +inf.
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -212,9 +213,18 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteParams p) {
 
 template <class T, bool BIAS>
 hipError_t launch_as(const RouteParams &p, hipStream_t s) {
+  // a launch has less than 2^32 lanes in all (the runtime starts the rest of them without an error): more tokens go one part after another
   auto go = [&](auto kernel, int lanes) {
-    kernel<<<dim3((unsigned)((p.tokens + 256 / lanes - 1) / (256 / lanes))), 256, 0, s>>>(p);
-    return hipGetLastError();
+    const int64_t each = ((int64_t)1 << 31) / lanes;
+    for (int64_t at = 0; at < p.tokens; at += each) {
+      RouteParams part = p;
+      part.tokens = std::min(each, p.tokens - at);
+      part.logits = (const T *)p.logits + at * p.ld, part.ids += at * p.ld_ids, part.weights += at * p.ld_weights;
+      kernel<<<dim3((unsigned)((part.tokens + 256 / lanes - 1) / (256 / lanes))), 256, 0, s>>>(part);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
   };
   if (p.experts <= 64) return go(moe_route_kernel<T, BIAS, 16, 4>, 16);
   if (p.experts <= 128) return go(moe_route_kernel<T, BIAS, 16, 8>, 16);
