@@ -130,6 +130,20 @@ def test_refused_calls(entry, args, change, status, says):
     assert says in N.lib().tts_last_error().decode()
 
 
+def test_experts_of_more_workgroups_than_a_launch_has_are_refused():
+    # tables of one matrix for all experts: 4096 slots in groups of their own, 2^24 columns
+    size, L = ctypes.c_size_t(), N.lib()
+    wide = dict(x=tensor(BF16, 4096, 8), ids=tensor(I32, 4096, 1))
+    up = tensor(BF16, 4096, 8, 1 << 24, stride=(0, 1 << 24, 1))
+    down = tensor(BF16, 4096, 1 << 24, 8, stride=(0, 8, 1))
+    assert L.tts_moe_experts_workspace(wide["x"], wide["ids"], up, down, 0, ctypes.byref(size)) == N.TTS_UNSUPPORTED
+    assert "more workgroups" in L.tts_last_error().decode()
+    up, down = tensor(BF16, 4096, 8, 8, stride=(0, 8, 1)), tensor(BF16, 4096, 8, 1 << 24, stride=(0, 1 << 24, 1))
+    assert L.tts_moe_experts_workspace(wide["x"], wide["ids"], up, down, 0, ctypes.byref(size)) == N.TTS_UNSUPPORTED
+    few = dict(x=tensor(BF16, 64, 8), ids=tensor(I32, 64, 1))
+    assert L.tts_moe_experts_workspace(few["x"], few["ids"], up, down, 0, ctypes.byref(size)) == N.TTS_OK
+
+
 def test_calls_for_no_tokens_do_nothing():
     L = N.lib()
     assert L.tts_moe_route(*route_args(logits=tensor(BF16, 0, 16, ptr=0), ids=tensor(I32, 0, 2, ptr=0), weights=tensor(F32, 0, 2, ptr=0))) == 0

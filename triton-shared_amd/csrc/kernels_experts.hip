@@ -592,6 +592,9 @@ int blocks_of(const ExpertMatrix &m, int64_t columns, int groups, int per_block)
 }
 
 int groups_of(const ExpertsParams &p) { return (int)std::min<int64_t>(p.tokens * p.top, p.experts); }
+int down_blocks(const ExpertsParams &p) {
+  return p.int8 ? blocks_of<true>(p.down, p.outputs, groups_of(p), 16) : blocks_of<false>(p.down, p.outputs, groups_of(p), 16);
+}
 int up_blocks(const ExpertsParams &p) {
   const int per_block = p.gated ? 8 : 16;  // columns of h
   return p.int8 ? blocks_of<true>(p.up, p.inner, groups_of(p), per_block) : blocks_of<false>(p.up, p.inner, groups_of(p), per_block);
@@ -599,7 +602,11 @@ int up_blocks(const ExpertsParams &p) {
 int h_cols(const ExpertsParams &p) { return up_blocks(p) * (p.gated ? 8 : 16); }
 
 // how many slabs of columns a workgroup does one after another: more, while that leaves enough workgroups
-int slabs_each(int slabs, int groups) { return std::max(1, std::min(8, slabs * groups / 768)); }
+int slabs_each(int slabs, int groups) { return (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)slabs * groups / 768)); }
+int64_t workgroups_of(int slabs, int groups) {
+  const int each = slabs_each(slabs, groups);
+  return (int64_t)((slabs + each - 1) / each) * groups;
+}
 
 // Rows of an expert at once (in 16s): nearly all of what an expert may have, if tokens pick them alike -- the mean and four times its root -- since
 // rows after those read the weights again; but not more, for registers (24 tokens, 16 experts of 2: 16 rows 170 us, 64 rows 195).
@@ -623,18 +630,17 @@ template <bool BF16, bool I8, bool MANY>
 hipError_t launch_experts_as(const ExpertsParams &p, hipStream_t s) {
   const Layout l = layout_of(p, h_cols(p));
   const int groups = groups_of(p), by_slot = groups < p.experts;
-  const int nb_up = up_blocks(p), nb_down = blocks_of<I8>(p.down, p.outputs, groups, 16);
+  const int nb_up = up_blocks(p), nb_down = down_blocks(p);
   auto up = [&](auto k1st, auto gated, auto mt, auto nb) {
-    const int each = slabs_each(l.slabs, groups);
     experts_up_kernel<BF16, I8, decltype(k1st)::value != 0, decltype(gated)::value != 0, decltype(mt)::value, decltype(nb)::value, WAVES>
-        <<<dim3((l.slabs + each - 1) / each * groups), 64 * WAVES, 0, s>>>(p, l, by_slot, l.slabs, each);
+        <<<dim3((unsigned)workgroups_of(l.slabs, groups)), 64 * WAVES, 0, s>>>(p, l, by_slot, l.slabs, slabs_each(l.slabs, groups));
     return hipGetLastError();
   };
   auto down = [&](auto k1st, auto mt, auto nb) {
     constexpr int width = 16 * decltype(nb)::value;
-    const int slabs = (int)((p.outputs + width - 1) / width), each = slabs_each(slabs, groups);
+    const int slabs = (int)((p.outputs + width - 1) / width);
     experts_down_kernel<BF16, I8, decltype(k1st)::value != 0, decltype(mt)::value, decltype(nb)::value, WAVES>
-        <<<dim3((slabs + each - 1) / each * groups), 64 * WAVES, 0, s>>>(p, l, by_slot, slabs, each);
+        <<<dim3((unsigned)workgroups_of(slabs, groups)), 64 * WAVES, 0, s>>>(p, l, by_slot, slabs, slabs_each(slabs, groups));
     return hipGetLastError();
   };
   auto with_rows = [&](auto mt) {
@@ -660,6 +666,12 @@ template hipError_t launch_experts_as<(TTS_EXPERTS_PART & 1) != 0, (TTS_EXPERTS_
 #else
 
 size_t experts_workspace_bytes(const ExpertsParams &p) { return layout_of(p, h_cols(p)).bytes; }
+
+bool experts_fit_a_grid(const ExpertsParams &p) {
+  const int down_cols = 16 * down_blocks(p);
+  const int64_t most = std::max(workgroups_of((int)((p.inner + h_cols(p) - 1) / h_cols(p)), groups_of(p)), workgroups_of((int)((p.outputs + down_cols - 1) / down_cols), groups_of(p)));
+  return most * (64 * WAVES) < (int64_t)1 << 32;
+}
 
 hipError_t launch_experts(const ExpertsParams &p, hipStream_t s) {
   auto of = [&](auto many) {

@@ -49,6 +49,7 @@ struct ExpertsParams {
   void *workspace;
 };
 size_t experts_workspace_bytes(const ExpertsParams &p);
+bool experts_fit_a_grid(const ExpertsParams &p);  // (a launch of 2^32 lanes and more starts only their remainder)
 hipError_t launch_experts(const ExpertsParams &p, hipStream_t s);
 
 constexpr int LORA_MAX_RANK = 1024;

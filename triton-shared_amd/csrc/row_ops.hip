@@ -31,7 +31,7 @@ const char *type_name(int dtype) {
 
 constexpr int64_t MOST_SIZE = (int64_t)1 << 30;  // of a dimension: sums of two fit 32 bits
 
-constexpr int64_t MOST_WIDTH = (int64_t)1 << 24;  // of a layer: its tiles times its slots fit a grid
+constexpr int64_t MOST_WIDTH = (int64_t)1 << 24;  // of a layer: its tiles fit 32 bits, and a token's sums a grid
 
 // one argument of a call, by its name
 struct Arg {
@@ -157,6 +157,7 @@ ExpertsParams experts_sizes(const tts_tensor *x_, const tts_tensor *ids_, const 
     unsupported(std::to_string(p.tokens) + " tokens of " + std::to_string(ids.size(1)) + " experts: more than " + std::to_string(EXPERTS_MAX_SLOTS) + " in all");
   p.top = (int)ids.size(1);
   p.up = matrix_of(w_up), p.down = matrix_of(w_down);
+  if (!experts_fit_a_grid(p)) unsupported(std::to_string(p.tokens * p.top) + " slots of " + std::to_string(p.inner) + " and " + std::to_string(p.outputs) + " columns: more workgroups than a launch has");
   return p;
 }
 
