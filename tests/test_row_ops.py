@@ -682,6 +682,27 @@ def test_gradients_are_refused_where_they_are_recorded():
 
 
 @pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad as fwd
+
+    a, e, logits = make_lora(4, 64, 64, 8, 2), make_experts(2, 2, 3, 64, 64, 64), gpu(3, 8)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for under in (torch.enable_grad, torch.no_grad):  # (no_grad is of the backward mode)
+            with under():
+                with pytest.raises(NotImplementedError, match="logits has a forward-mode tangent"):
+                    ops.moe_route(dual(logits), 2)
+                with pytest.raises(NotImplementedError, match="weights has a forward-mode tangent"):
+                    ops.moe_experts(e["x"], e["ids"], dual(e["weights"]), e["w_up"], e["w_down"])
+                with pytest.raises(NotImplementedError, match="scales has a forward-mode tangent"):
+                    ops.lora_add(a["base"], a["x"], a["a"], a["b"], a["ids"], scales=dual(a["scales"]))
+                with pytest.raises(NotImplementedError, match="out has a forward-mode tangent"):
+                    ops.lora_add(a["base"], a["x"], a["a"], a["b"], a["ids"], out=dual(torch.empty_like(a["base"])))
+        inside = ops.moe_route(logits, 2)   # without one: as ever
+    assert all(torch.equal(x, y) for x, y in zip(inside, ops.moe_route(logits, 2)))
+
+
+@pytest.mark.gpu
 def test_python_arguments_are_checked():
     a = make_experts(2, 2, 3, 64, 64, 64)
     call = lambda **kw: ops.moe_experts(**({k: v for k, v in a.items()} | kw))  # noqa: E731

@@ -7,11 +7,12 @@
 They are hand-written kernels behind the C ABI (include/tts_hip.h: tts_moe_route, tts_moe_experts, tts_lora_add), for code that
 calls them beside its Triton kernels: on the current stream of their tensors' device, asynchronous, capturable into a graph.
 Wrong arguments raise ValueError or TypeError, what is not implemented NotImplementedError, failing HIP calls RuntimeError.
-They have no backward pass: tensors that require gradients are refused where gradients are recorded.
+They have no derivatives: tensors that require gradients are refused where gradients are recorded, and those with a forward-mode tangent anywhere.
 """
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -34,6 +35,8 @@ def _describe(name, t, device):
         raise ValueError(f"{name} has {t.dim()} dimensions")
     if t.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{name} requires a gradient, and this operator has no backward pass: call it under torch.no_grad()")
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} has a forward-mode tangent, which this operator does not carry on")
     d = _native.TtsTensor(t.data_ptr(), _DTYPES[t.dtype], t.dim())
     d.shape[:t.dim()] = t.shape
     d.stride[:t.dim()] = t.stride()
@@ -55,6 +58,12 @@ def _native_calls():
                          torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, *_DTYPES, torch.Tensor, torch.nn.Parameter, _native._raise)
         _fast = module
     return _fast
+
+
+def _ordinary():
+    """The launch extension's calls, or False: without it, and inside a level of forward-mode derivatives, since it does not look for tangents."""
+    fast = _native_calls() if _fast is None else _fast
+    return fast if getattr(forward_ad, "_current_level", 0) < 0 else False
 
 
 def _device_of(name, t):
@@ -95,7 +104,7 @@ def moe_route(logits, k, scoring="softmax", bias=None, renormalize=True, scale=1
     than k others are left, ids are -1 and weights 0.  A row that holds a NaN gets weights of NaN, as does the softmax of
     one that holds +inf.
     """
-    fast = _native_calls() if _fast is None else _fast
+    fast = _ordinary()
     if fast:
         made = fast.moe_route(logits, k, _SCORING.get(scoring), bias, renormalize, scale)
         if made is not None:
@@ -122,7 +131,7 @@ def moe_experts(x, ids, weights, w_up, w_down, s_up=None, s_down=None, activatio
     Either dimension of a matrix may be the contiguous one: pass `w.transpose(1, 2)` of weights stored as [E, outputs, inputs].
     An id outside [0, E) contributes nothing.  `out` may be x.
     """
-    fast = _native_calls() if _fast is None else _fast
+    fast = _ordinary()
     if fast:
         made = fast.moe_experts(x, ids, weights, w_up, w_down, s_up, s_down, _ACTIVATION.get(activation), gated, out)
         if made is not None:
@@ -146,7 +155,7 @@ def lora_add(base, x, a, b, ids, scales=None, out=None):
     base [T, N], x [T, K], a [n, r, K], b [n, N, r] (as nn.Linear stores such weights), all float16 or all bfloat16; ids [T] int32, scales [n] float32
     or None for 1.  `out` may be base itself, for an update in place.  A prompt's rows next to each other share the reading of their adapter.
     """
-    fast = _native_calls() if _fast is None else _fast
+    fast = _ordinary()
     if fast:
         made = fast.lora_add(base, x, a, b, ids, scales, out)
         if made is not None:
