@@ -703,6 +703,28 @@ def test_forward_mode_derivatives_are_refused():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ordinary", [True, False])
+def test_autograd_notices_that_out_was_written(ordinary, monkeypatch):
+    if not ordinary:  # the calls that the launch extension leaves to Python
+        monkeypatch.setattr(ops, "_fast", False)
+    a, e = make_lora(4, 64, 64, 8, 2), make_experts(2, 2, 3, 64, 64, 64)
+    for write in (lambda out: ops.lora_add(out, a["x"], a["a"], a["b"], a["ids"], out=out), lambda out: ops.moe_experts(e["x"], e["ids"], e["weights"], e["w_up"], e["w_down"], out=out[:2])):
+        factor = torch.ones(64, device="cuda", requires_grad=True)
+        saved = a["base"].clone()
+        y = (saved * factor).sum()
+        write(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        out = torch.empty_like(a["base"])
+        assert ops.lora_add(a["base"], a["x"], a["a"], a["b"], a["ids"], out=out) is out
+    version = a["base"]._version
+    with pytest.raises(ValueError):         # a refused call has written nothing
+        ops.lora_add(a["base"], a["x"], a["a"], a["b"], a["ids"].float(), out=a["base"])
+    assert a["base"]._version == version
+
+
+@pytest.mark.gpu
 def test_python_arguments_are_checked():
     a = make_experts(2, 2, 3, 64, 64, 64)
     call = lambda **kw: ops.moe_experts(**({k: v for k, v in a.items()} | kw))  # noqa: E731

@@ -80,6 +80,12 @@ def _choice(name, value, table):
     return table[value]
 
 
+def _written(out):
+    """`out`, of which autograd knows now that it has changed: a backward pass that has saved it raises."""
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
 def _call(entry, device, *args):
     with torch.cuda.device(device):
         status = entry(*args, torch.cuda.current_stream(device).cuda_stream)
@@ -135,16 +141,15 @@ def moe_experts(x, ids, weights, w_up, w_down, s_up=None, s_down=None, activatio
     if fast:
         made = fast.moe_experts(x, ids, weights, w_up, w_down, s_up, s_down, _ACTIVATION.get(activation), gated, out)
         if made is not None:
-            return made
+            return made if out is None else _written(out)
     device = _device_of("x", x)
     act = _choice("activation", activation, _ACTIVATION)
     dx, di, du, dd = _describe("x", x, device), _describe("ids", ids, device), _describe("w_up", w_up, device), _describe("w_down", w_down, device)
     work = _workspace(_native.lib().tts_moe_experts_workspace, device, dx, di, du, dd, bool(gated))
-    if out is None:
-        out = torch.empty(x.shape[0], w_down.shape[2], dtype=x.dtype, device=device)
+    given, out = out, torch.empty(x.shape[0], w_down.shape[2], dtype=x.dtype, device=device) if out is None else out
     _call(_native.lib().tts_moe_experts, device, dx, di, _describe("weights", weights, device), du, _describe("s_up", s_up, device), dd, _describe("s_down", s_down, device), act,
           bool(gated), _describe("out", out, device), work.data_ptr(), work.numel())
-    return out
+    return out if given is None else _written(out)
 
 
 def lora_add(base, x, a, b, ids, scales=None, out=None):
@@ -159,12 +164,11 @@ def lora_add(base, x, a, b, ids, scales=None, out=None):
     if fast:
         made = fast.lora_add(base, x, a, b, ids, scales, out)
         if made is not None:
-            return made
+            return made if out is None else _written(out)
     device = _device_of("base", base)
     db, dx, da, dl = _describe("base", base, device), _describe("x", x, device), _describe("a", a, device), _describe("b", b, device)
     work = _workspace(_native.lib().tts_lora_add_workspace, device, dx, dl)
-    if out is None:
-        out = torch.empty_like(base, memory_format=torch.contiguous_format)
+    given, out = out, torch.empty_like(base, memory_format=torch.contiguous_format) if out is None else out
     _call(_native.lib().tts_lora_add, device, db, dx, da, dl, _describe("ids", ids, device), _describe("scales", scales, device), _describe("out", out, device), work.data_ptr(),
           work.numel())
-    return out
+    return out if given is None else _written(out)
