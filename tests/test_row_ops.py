@@ -748,6 +748,14 @@ def test_python_arguments_are_checked():
 
 
 @pytest.mark.gpu
+def test_route_refuses_more_choices_than_experts_before_it_allocates():
+    logits = gpu(16384, 8)
+    for k in (9, 10 ** 9, 10 ** 30):        # (a table of 10^9 choices would be 65 TB)
+        with pytest.raises(ValueError, match=f"k is {k}"):
+            ops.moe_route(logits, k)
+
+
+@pytest.mark.gpu
 def test_results_do_not_change_from_call_to_call():
     e, l = make_experts(24, 4, 8, 256, 192, 256), make_lora(70, 256, 256, 16, 9)
     first = None

@@ -276,7 +276,7 @@ PyObject *op_route(PyObject *, PyObject *const *a, Py_ssize_t n) {
   int64_t k = 0, scoring = 0;
   if (!o.ok || !PyLong_CheckExact(a[1]) || !to_int64(a[1], &k) || k < 1 || !to_int64(a[2], &scoring) || !PyBool_Check(a[4]) || !PyFloat_CheckExact(a[5])) return not_ordinary();
   const tts_tensor *l = o.describe(a[0], logits), *b = o.describe(a[3], bias);
-  if (!l || !o.ok || l->rank != 2) return not_ordinary();
+  if (!l || !o.ok || l->rank != 2 || k > logits.shape[1]) return not_ordinary();
   Ref made_ids(o.make(a[0], logits.shape[0], k, g_ops.dtypes[TTS_I32], ids)), made_weights(o.make(a[0], logits.shape[0], k, g_ops.dtypes[TTS_F32], weights));
   if (!o.ok) return not_ordinary();
   const bool renormalize = a[4] == Py_True;

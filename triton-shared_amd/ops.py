@@ -118,8 +118,8 @@ def moe_route(logits, k, scoring="softmax", bias=None, renormalize=True, scale=1
     device = _device_of("logits", logits)
     if logits.dim() != 2:
         raise ValueError(f"logits have {logits.dim()} dimensions, not 2")
-    if k < 1:
-        raise ValueError(f"k is {k}")
+    if k < 1 or k > logits.shape[1]:
+        raise ValueError(f"k is {k}" if k < 1 else f"k is {k}, and there are {logits.shape[1]} experts")
     ids = torch.empty(logits.shape[0], k, dtype=torch.int32, device=device)
     weights = torch.empty(logits.shape[0], k, dtype=torch.float32, device=device)
     _call(_native.lib().tts_moe_route, device, _describe("logits", logits, device), _describe("bias", bias, device), _choice("scoring", scoring, _SCORING), bool(renormalize),
