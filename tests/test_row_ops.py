@@ -458,6 +458,28 @@ def test_experts_with_several_slabs_per_workgroup(I, O, dtype, weights, order):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [256, 100])      # up to 64, and up to 32, rows of an expert at once
+@pytest.mark.parametrize("H,I,O,gated", [(808, 520, 1032, True), (72, 1544, 72, True), (72, 72, 3112, True), (72, 1032, 72, False)])
+@pytest.mark.parametrize("dtype,weights", [("bf16", None), ("fp16", None), ("bf16", "int8"), ("fp16", "int8")])
+@pytest.mark.parametrize("order", ["in", "out"])
+def test_experts_of_many_rows_in_wide_tiles(order, dtype, weights, H, I, O, gated, T):
+    a = make_experts(T, 5, 64, H, I, O, dtype, weights, order, order, gated, seed=T)
+    a["ids"][:70, 0] = 7                        # an expert whose rows take several turns
+    got = ops.moe_experts(a["x"], a["ids"], a["weights"], a["w_up"], a["w_down"], s_up=a["s_up"], s_down=a["s_down"], gated=gated)
+    rows = [0, 15, 16, 17, 31, 32, 33, 63, 64, 69, 70, T - 2, T - 1]
+    part = {n: a[n][rows] for n in ("x", "ids", "weights")}
+    want, lim = experts_exact(**part, w_up=a["w_up"], w_down=a["w_down"], s_up=a["s_up"], s_down=a["s_down"], activation="silu", gated=gated)
+    off = (got[rows].double() - want).abs()
+    assert bool((off <= lim).all()), f"off by {(off / lim).max().item():.2f} of what is allowed"
+    # all rows, against calls of a few tokens
+    for at in range(0, T, 50):
+        few = [a[n][at:at + 50] for n in ("x", "ids", "weights")]
+        again = ops.moe_experts(*few, a["w_up"], a["w_down"], s_up=a["s_up"], s_down=a["s_down"], gated=gated)
+        # (both within `lim` of the same values, and no row's `lim` is twice the largest of the rows above: these are alike)
+        assert bool(((got[at:at + 50].double() - again.double()).abs() <= 4 * lim.max()).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_experts_ids_outside_repeated_and_one_for_all(dtype):
     a = make_experts(50, 3, 6, 128, 96, 128, dtype)
@@ -596,6 +618,14 @@ def check_lora(a, **kw):
                                             (1100, 96, 130, 16, 6, 90), (1037, 130, 96, 24, 9, 1), (2048, 64, 512, 64, 3, 700), (1500, 257, 77, 130, 4, 333)])
 def test_lora(T, K, O, r, n, runs, dtype):
     check_lora(make_lora(T, K, O, r, n, dtype, runs, seed=T + r))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("r", [2, 4, 7])
+@pytest.mark.parametrize("T,O,runs", [(20, 4096, 1), (20, 515, 1), (1100, 1040, 90), (1100, 515, 1)])
+def test_lora_of_ranks_below_an_octet(T, O, runs, r, dtype):
+    check_lora(make_lora(T, 96, O, r, 5, dtype, runs, seed=T + O + r))
 
 
 @pytest.mark.gpu
