@@ -426,43 +426,43 @@ __global__ __launch_bounds__(64 * WAVES) void experts_up_kernel(ExpertsParams p,
       rows[mc.value] = (const char *)p.x + (int64_t)((u32)list[r] / (u32)p.top) * p.ld_x * 2;
     });
     for (int sl = slab; sl < last_slab; sl++) {
-    const int tile0 = sl * HC;
-    f32x4 acc[MT][NB];
-    each<0, MT * NB>([&](auto ic) __attribute__((always_inline)) { acc[ic.value / NB][ic.value % NB] = (f32x4){0.f, 0.f, 0.f, 0.f}; });
-    product.template rows<R, MT>(acc, rows, 0, one);
-    // the next columns' (or rows') weights are on their way while these sums are added
-    if (sl + 1 < last_slab) product.begin(tile0 + HC);
-    else if (r0 + 16 * MT < n) product.begin(slab * HC);
-    each<0, MT>([&](auto mc) __attribute__((always_inline)) {
-      constexpr int m = decltype(mc)::value, TPR = 4 * WAVES;  // threads per row
-      put_sums<K1ST, NB>(red + wave * 16 * PITCH, PITCH, acc[m], lane);
-      __syncthreads();
-      const int r = tid / TPR, part = tid % TPR;
-      const int slot = r0 + 16 * m + r < n ? list[r0 + 16 * m + r] : -1;
-      float most = 0.f;
-      for (int j = part; j < HC; j += TPR) {
-        // the column that place j holds
-        const int col = W::column(tile0, j / W::GROUP, inner) + j % W::GROUP;
-        float gate = 0.f, up = 0.f;
-        for (int q = 0; q < WAVES; q++) {
-          gate += red[(q * 16 + r) * PITCH + j];
-          if (GATED) up += red[(q * 16 + r) * PITCH + HC + j];
+      const int tile0 = sl * HC;
+      f32x4 acc[MT][NB];
+      each<0, MT * NB>([&](auto ic) __attribute__((always_inline)) { acc[ic.value / NB][ic.value % NB] = (f32x4){0.f, 0.f, 0.f, 0.f}; });
+      product.template rows<R, MT>(acc, rows, 0, one);
+      // the next columns' (or rows') weights are on their way while these sums are added
+      if (sl + 1 < last_slab) product.begin(tile0 + HC);
+      else if (r0 + 16 * MT < n) product.begin(slab * HC);
+      each<0, MT>([&](auto mc) __attribute__((always_inline)) {
+        constexpr int m = decltype(mc)::value, TPR = 4 * WAVES;  // threads per row
+        put_sums<K1ST, NB>(red + wave * 16 * PITCH, PITCH, acc[m], lane);
+        __syncthreads();
+        const int r = tid / TPR, part = tid % TPR;
+        const int slot = r0 + 16 * m + r < n ? list[r0 + 16 * m + r] : -1;
+        float most = 0.f;
+        for (int j = part; j < HC; j += TPR) {
+          // the column that place j holds
+          const int col = W::column(tile0, j / W::GROUP, inner) + j % W::GROUP;
+          float gate = 0.f, up = 0.f;
+          for (int q = 0; q < WAVES; q++) {
+            gate += red[(q * 16 + r) * PITCH + j];
+            if (GATED) up += red[(q * 16 + r) * PITCH + HC + j];
+          }
+          if (I8) {
+            gate *= scales[col];
+            if (GATED) up *= scales[inner + col];
+          }
+          const float h = GATED ? activate(p.activation, gate) * up : activate(p.activation, gate);
+          most = fmaxf(most, fabsf(h));
+          if (slot >= 0 && col >= tile0) put_h<BF16>(l, slot, col, h);
         }
-        if (I8) {
-          gate *= scales[col];
-          if (GATED) up *= scales[inner + col];
+        if (slot >= 0 && tile0 + HC >= inner && part < 8 && inner + part < l.pitch_h) put_h<BF16>(l, slot, inner + part, 0.f);
+        if (!BF16) {
+          for (int d = 1; d < TPR; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+          if (slot >= 0 && part == 0) l.row_max[(int64_t)slot * l.slabs + sl] = most;
         }
-        const float h = GATED ? activate(p.activation, gate) * up : activate(p.activation, gate);
-        most = fmaxf(most, fabsf(h));
-        if (slot >= 0 && col >= tile0) put_h<BF16>(l, slot, col, h);
-      }
-      if (slot >= 0 && tile0 + HC >= inner && part < 8 && inner + part < l.pitch_h) put_h<BF16>(l, slot, inner + part, 0.f);
-      if (!BF16) {
-        for (int d = 1; d < TPR; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-        if (slot >= 0 && part == 0) l.row_max[(int64_t)slot * l.slabs + sl] = most;
-      }
-      __syncthreads();
-    });
+        __syncthreads();
+      });
     }
   };
   for (int r0 = 0; r0 < n;)
@@ -523,32 +523,32 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(ExpertsParams 
       weight[mc.value] = p.weights[(int64_t)t * p.ld_weights + (slot - (int)t * p.top)];
     });
     for (int sl = slab; sl < last_slab; sl++) {
-    const int tile0 = sl * COLS<NB>;
-    f32x4 acc[MT][NB];
-    each<0, MT * NB>([&](auto ic) __attribute__((always_inline)) { acc[ic.value / NB][ic.value % NB] = (f32x4){0.f, 0.f, 0.f, 0.f}; });
-    product.template rows<R, MT>(acc, rows, l.plane, scale);
-    // the next columns' (or rows') weights are on their way while these sums are added
-    if (sl + 1 < last_slab) product.begin(tile0 + COLS<NB>);
-    else if (r0 + 16 * MT < n) product.begin(slab * COLS<NB>);
-    each<0, MT>([&](auto mc) __attribute__((always_inline)) {
-      constexpr int m = decltype(mc)::value;
-      put_sums<K1ST, NB>(red + wave * 16 * PITCH, PITCH, acc[m], lane);
-      __syncthreads();
-      const int r = tid / TPR;
-      if (r0 + 16 * m + r < n) {
-        const int slot = list[r0 + 16 * m + r];
-        const float back = BF16 ? 1.f : 1.f / row_scale[16 * m + r];  // (a power of two)
-        for (int j = tid % TPR; j < COLS<NB>; j += TPR) {
-          const int col = W::column(tile0, j / W::GROUP, outputs) + j % W::GROUP;
-          float v = 0.f;
-          for (int q = 0; q < WAVES; q++) v += red[(q * 16 + r) * PITCH + j];
-          if (!BF16) v *= back;
-          if (I8) v *= scales[col];
-          l.partial[(int64_t)slot * outputs + col] = v * weight[m];
+      const int tile0 = sl * COLS<NB>;
+      f32x4 acc[MT][NB];
+      each<0, MT * NB>([&](auto ic) __attribute__((always_inline)) { acc[ic.value / NB][ic.value % NB] = (f32x4){0.f, 0.f, 0.f, 0.f}; });
+      product.template rows<R, MT>(acc, rows, l.plane, scale);
+      // the next columns' (or rows') weights are on their way while these sums are added
+      if (sl + 1 < last_slab) product.begin(tile0 + COLS<NB>);
+      else if (r0 + 16 * MT < n) product.begin(slab * COLS<NB>);
+      each<0, MT>([&](auto mc) __attribute__((always_inline)) {
+        constexpr int m = decltype(mc)::value;
+        put_sums<K1ST, NB>(red + wave * 16 * PITCH, PITCH, acc[m], lane);
+        __syncthreads();
+        const int r = tid / TPR;
+        if (r0 + 16 * m + r < n) {
+          const int slot = list[r0 + 16 * m + r];
+          const float back = BF16 ? 1.f : 1.f / row_scale[16 * m + r];  // (a power of two)
+          for (int j = tid % TPR; j < COLS<NB>; j += TPR) {
+            const int col = W::column(tile0, j / W::GROUP, outputs) + j % W::GROUP;
+            float v = 0.f;
+            for (int q = 0; q < WAVES; q++) v += red[(q * 16 + r) * PITCH + j];
+            if (!BF16) v *= back;
+            if (I8) v *= scales[col];
+            l.partial[(int64_t)slot * outputs + col] = v * weight[m];
+          }
         }
-      }
-      __syncthreads();
-    });
+        __syncthreads();
+      });
     }
   };
   for (int r0 = 0; r0 < n;)
@@ -584,7 +584,11 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(ExpertsParams p, const
 // The blocks of 16 columns per workgroup.  Wide tiles read the rows again less often (256 tokens, 64 experts of 4096 x 1536: 559 us of eight blocks of
 // contiguous k, 597 of four) and, with contiguous columns, whole cache lines of each row of k (16 experts of int8: 184 us of sixteen, 240 of
 // eight); half as wide where that leaves too few workgroups to read at the memory's pace (one token, 8 experts of 2048 x 768: contiguous k 30 us of
-// four, 42 of eight; columns 34 of four, 38 of eight, of int8 33 and 51).
+// four, 42 of eight; columns 34 of four, 38 of eight, of int8 33 and 51).  Near the borders, layers of 2048 in and out, us wide and half as wide: contiguous
+// k, 256 workgroups 44.5 and 43.1, 512 79.7 and 83.2, 1024 142.7 and 138.6, of int8 33.4 and 31.4, 55.6 and 52.5, 97.7 and 89.4; columns, 64 workgroups
+// 31.7 and 29.1, 128 36.1 and 35.3, 256 49.2 and 63.1, of int8 40.7 and 32.5, 46.0 and 39.7, 57.3 and 68.5.
+// int8 tiles of sixteen blocks with 64 rows at once have more sums than registers (60 to 87 spill).  They are ahead all the same where an expert's rows
+// are one turn (128 tokens, 4 of 32 experts of 4096 x 4096: 392 us, 579 of eight), not where they are several (256 tokens, 2 of 8 of 4096 x 2048: 252, 166).
 template <bool I8>
 int blocks_of(const ExpertMatrix &m, int64_t columns, int groups, int per_block) {
   const int most = m.w_k != 1 && I8 ? 16 : 8;
@@ -601,7 +605,8 @@ int up_blocks(const ExpertsParams &p) {
 }
 int h_cols(const ExpertsParams &p) { return up_blocks(p) * (p.gated ? 8 : 16); }
 
-// how many slabs of columns a workgroup does one after another: more, while that leaves enough workgroups
+// How many slabs of columns a workgroup does one after another: more, while that leaves enough workgroups.  (256 tokens, 6 of 64 experts of 4096 x 1536: 538 us;
+// 637 of twice as many slabs, 545 of half as many or one.  32 tokens, 4 of 64 of 2048 x 2048, contiguous columns: 277, 264 and 291, contiguous k 279, 296 and 275.)
 int slabs_each(int slabs, int groups) { return (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)slabs * groups / 768)); }
 int64_t workgroups_of(int slabs, int groups) {
   const int each = slabs_each(slabs, groups);

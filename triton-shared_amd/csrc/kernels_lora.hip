@@ -7,8 +7,9 @@
 // v is summed and kept in 32 bits, in slices of the inputs that kernel 2 adds as it reads them; it enters the second product as
 // two 16-bit parts (row_device.h).
 // What has to move is x, base and out once and the adapters.  What bounds it: few rows, the launches and chains of loads (one row of 4096 x 4096, rank
-// 16: 4 + 7 us; 64 rows with an adapter each, 4096 x 8192: 10 + 15 us, up to 16 adapters in turn per tile, eight loads ahead); prompts, the chain of
-// load, product and store in two workgroups per CU (8192 rows, rank 64: 37 us for 67 MB of x, 60 us for 134 MB of base and out, 2.2 TB/s).
+// 16: 4 + 7 us; 64 rows with an adapter each, 4096 x 8192: 10 + 15 us, up to 16 adapters in turn per tile, eight loads ahead); prompts of 8192 rows, rank 64:
+// kernel 1 is one round of one workgroup per CU (64 rows take the registers of a SIMD for one wavefront), whose first loads and last sums nothing
+// overlaps, 37 us for 67 MB of x; kernel 2, two workgroups per CU, reads B for every 32 rows, 134 MB from L2 beside as much of base and out, 60 us.
 #include <algorithm>
 #include <cmath>
 
@@ -53,13 +54,13 @@ __device__ __forceinline__ int row_id(const LoraParams &p, int64_t row) {
   return (u32)id < (u32)p.adapters ? id : -1;
 }
 
-// eight 16-bit elements from any element's address, the first `valid` of them; zero behind
+// eight 16-bit elements from any element's address
 __device__ __forceinline__ uint4 octet(const char *p) {
   uint4 v;
   __builtin_memcpy(&v, p, 16);
   return v;
 }
-// How rows end.  (The checks at every load would be most of a kernel's code, and a launch for few rows waits for its code.)
+// ... the first `valid` of them, zeros behind, by how rows end.  (The checks at every load would be most of a kernel's code, and a launch for few rows waits for its code.)
 enum Ends { EXACT = 3,  // with a whole step of 64
             EVEN = 0,   // with a whole octet
             LONG = 1,   // anywhere, at least eight elements from their beginning: the last octet's load is moved back to end with the row
@@ -359,7 +360,10 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p, Shape sh
 constexpr int CUS = 256;
 
 // Rows of a workgroup.  Few rows: as many workgroups as there can be.  Of prompts kernel 1 takes 64 (an adapter is read again for every
-// tile: 8192 rows, rank 64: 36 us of 64, 43 of 32) and kernel 2 32 (it holds base and the sums: 59 us of 32, 82 of 64).
+// tile: 8192 rows, rank 64: 36 us of 64, 43 of 32) and kernel 2 32 (it holds base and the sums: 59 us of 32, 82 of 64).  Both kernels of 4096 x 4096, us of
+// 16 rows and of 64 / 32: rank 16, one adapter, 512 rows 12 and 15, 1024 rows 18 and 19, 2048 rows 25 and 24, 4096 rows 45 and 39; 64 adapters row by
+// row 30 and 52, 47 and 58, 80 and 95, 148 and 170; rank 64, one adapter 18 and 21, 26 and 24, 40 and 32, 71 and 47; 64 adapters 71 and 103, 125 and 129,
+// 239 and 229, 467 and 434.
 bool many_rows(const LoraParams &p) { return p.tokens > 1024; }
 
 Shape shape_of(const LoraParams &p) {

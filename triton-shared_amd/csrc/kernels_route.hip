@@ -93,8 +93,8 @@ constexpr float NO_SCORE = -745.f;
 // G lanes per token; lane i of them holds experts i, i + G, ... (N of them).  Which expert is chosen shows whole, so where scores get a bias
 // the choice is that of c in 64 bits: 32 bits decide it unless two that matter are near each other, which is seldom (a token in a thousand of
 // the one measured); then the candidates' c is computed in 64 bits and the choice made again.
-// What bounds it: one token 4.7 us, a launch and a chain of two reductions per choice; 16384 tokens of 256 fp32 logits 10 us without a bias (17 MB, 3.3
-// at a copy's rate: a choice is some 160 instructions of four tokens' lanes), 20 with one, of which the last wavefront's second choice is
+// What bounds it: one token 4.5 us, a launch and a chain of two reductions per choice; 16384 tokens of 256 fp32 logits 11 us without a bias (17 MB, 3.3
+// at a copy's rate: a choice is some 160 instructions of four tokens' lanes), 21 with one, of which the last wavefront's second choice is
 // half: it starts on code that is not in the instruction cache yet.
 template <class T, bool BIAS, int G, int N>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteParams p) {
