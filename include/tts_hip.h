@@ -149,7 +149,7 @@ tts_status tts_moe_experts(const tts_tensor *x, const tts_tensor *ids, const tts
 /* Low-rank adapters of many requests:
  *   out[t] = base[t] + scales[d] * (x[t] a[d]^T) b[d]^T,  d = ids[t];  out[t] = base[t], bit for bit, where d is not in [0, n).
  * base and out [T, N], x [T, K], a [n, r, K], b [n, N, r], all f16 or all bf16, the last dimension with stride 1; ids [T] i32, scales [n]
- * f32 or NULL (1); r <= 1024.  out may be base itself; otherwise it shares no memory with the inputs.  One request's adapter
+ * f32 or NULL (1); r <= 1024, T <= 2097120.  out may be base itself; otherwise it shares no memory with the inputs.  One request's adapter
  * (an infinity in it, say) does not reach another's rows.  Rows of one adapter next to each other read it once per 16 rows; in calls of more
  * than 1024 rows, a once per 64 and b once per 32. */
 tts_status tts_lora_add_workspace(const tts_tensor *x, const tts_tensor *b, size_t *bytes);

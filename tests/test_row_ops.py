@@ -151,6 +151,13 @@ def test_calls_for_no_tokens_do_nothing():
     assert L.tts_lora_add(*lora_args(base=tensor(F16, 0, 96, ptr=0), x=tensor(F16, 0, 64, ptr=0), ids=tensor(I32, 0, ptr=0), out=tensor(F16, 0, 96, ptr=0), work=None, bytes=0)) == 0
 
 
+def test_adapters_of_more_rows_than_a_grid_has_are_refused():
+    size, L = ctypes.c_size_t(), N.lib()
+    assert L.tts_lora_add_workspace(tensor(BF16, 2097120, 64), tensor(BF16, 8, 64, 16), ctypes.byref(size)) == N.TTS_OK
+    assert L.tts_lora_add_workspace(tensor(BF16, 2097121, 64), tensor(BF16, 8, 64, 16), ctypes.byref(size)) == N.TTS_UNSUPPORTED
+    assert "2097121 rows" in L.tts_last_error().decode()
+
+
 def test_columns_of_one_buffer_are_told_apart():
     # out and x side by side in rows of one buffer do not overlap; moved by one element they do
     x = tensor(F16, 4, 64, stride=(256, 1), ptr=FAR[1] + 2 * 96)

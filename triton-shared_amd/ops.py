@@ -158,7 +158,7 @@ def lora_add(base, x, a, b, ids, scales=None, out=None):
         out[t] = base[t] + scales[d] * (x[t] a[d]^T) b[d]^T,   d = ids[t];   out[t] = base[t] where d is not in [0, n)
 
     base [T, N], x [T, K], a [n, r, K], b [n, N, r] (as nn.Linear stores such weights), all float16 or all bfloat16; ids [T] int32, scales [n] float32
-    or None for 1.  `out` may be base itself, for an update in place.  A prompt's rows next to each other share the reading of their adapter.
+    or None for 1; T up to 2097120.  `out` may be base itself, for an update in place.  A prompt's rows next to each other share the reading of their adapter.
     """
     fast = _ordinary()
     if fast:
