@@ -156,6 +156,52 @@ tts_status tts_lora_add_workspace(const tts_tensor *x, const tts_tensor *b, size
 tts_status tts_lora_add(const tts_tensor *base, const tts_tensor *x, const tts_tensor *a, const tts_tensor *b, const tts_tensor *ids,
                         const tts_tensor *scales, const tts_tensor *out, void *workspace, size_t bytes, void *stream);
 
+/* ---- The attention part of a decode step over a cache held in 4 bits: page_slots -> qk_norm_rope -> kv4_write -> kv4_attention.  No counterpart in
+ * the reference.  They behave as the operators above: asynchronous on `stream`, nothing allocated or compiled, scratch memory from the caller, arguments
+ * checked on the host, what memory holds (lengths, pages, slots, positions) on the device.  Vectors have stride 1; the last dimension of what is a matrix or more has, too.
+ * A step has T rows, the new tokens of one request after another; rows behind the last request's (a batch padded to what a graph was captured for) have no request. */
+
+/* Block tables and slot maps.  table [B, M] i32: the pages of each request, in order; lengths [B] i32: the tokens that it has after this step, fresh [B]
+ * i32: how many of them are new, its last ones (held between 0 and its length); free [F] i32: a stack of free pages, of which the first count[0] are on it, the last of them the
+ * top.  B <= 4096.  Requests take the pages that they lack (to ceil(length / page), at most M) from the top of the stack, the first request first, each in the order of its
+ * columns; those are written into the table, and nothing else of it; where the stack has run out, -1.  Written besides: slots [T] i32, table[b][position / page] * page + position %
+ * page of each row, or -1 where there is no such page; positions [T]; owners [T], the row's request; -1 in all three for rows of no request; starts [B + 1], where the
+ * requests' rows begin, and their end; left [1], how many pages are on the stack now.  If the requests have more than T rows, those behind have no slots here.  What is
+ * written shares no memory with what is read. */
+tts_status tts_page_slots(const tts_tensor *table, const tts_tensor *lengths, const tts_tensor *fresh, const tts_tensor *free, const tts_tensor *count, int page,
+                          const tts_tensor *slots, const tts_tensor *positions, const tts_tensor *owners, const tts_tensor *starts, const tts_tensor *left, void *stream);
+
+/* Norms of queries and keys for each head, and the rotation by position.  q [T, Hq, D], k [T, Hk, D] (f32, f16, bf16; D even, <= 512), tokens and heads any distance
+ * apart (columns of one projection's rows, say).  Of each head y = x / sqrt(mean(x^2) + eps) * w, w_q and w_k [D] of q's type or f32 (both NULL: y = x); then of its first R
+ * elements pairs (a, b) become (a cos - b sin, b cos + a sin): pair n is elements n and n + R / 2, or 2 n and 2 n + 1 if `interleaved`; cos_sin [P, R] f32 holds the cosines of a
+ * position's R / 2 angles, then their sines; positions [T] i32.  Nothing of a row whose position is not in [0, P) is written, or zeros if `clear`.
+ * Sums and products in 32 bits, rounded once.  q_out may be q itself and k_out k; otherwise what is written shares no memory with what is read. */
+tts_status tts_qk_norm_rope(const tts_tensor *q, const tts_tensor *k, const tts_tensor *positions, const tts_tensor *cos_sin, const tts_tensor *w_q, const tts_tensor *w_k,
+                            double eps, int interleaved, int clear, const tts_tensor *q_out, const tts_tensor *k_out, void *stream);
+
+/* The cache [pages, Hk, page * (D + 8) / 2], f16 or bf16: for each page and head the keys and values of `page` tokens (a multiple of 16), of each element 4
+ * bits and of each token's key and value a step and a lowest value of the cache's type; pages * page <= 2^31 - 1.  D is a multiple of 32 up to 256.  The last dimension has stride 1,
+ * pages and heads are multiples of 16 bytes apart (8 elements).  Its inner layout is the library's own.
+ * An element x of a head with lowest value l and largest h is held as c * s + l, s = (h - l) / 15 in 32 bits rounded to the type, c = how many of the borders
+ * (n + 1/2) s, n = 0 .. 14, x - l is above.  A head that holds a NaN or an infinity, or whose h - l is not finite in 32 bits, is held as NaN.
+ * write: k, v [T, Hk, D] of the cache's type into slots [T] i32 (page * tokens of a page + place in it); a row whose slot is not in the cache is not written.  The slots in
+ * the cache are distinct: of two rows with the same one, parts of either are there afterwards.
+ * read: what the slots hold, code * step + lowest rounded to the type; zeros for a slot that is not in the cache. */
+tts_status tts_kv4_write(const tts_tensor *cache, const tts_tensor *k, const tts_tensor *v, const tts_tensor *slots, void *stream);
+tts_status tts_kv4_read(const tts_tensor *cache, const tts_tensor *slots, const tts_tensor *k, const tts_tensor *v, void *stream);
+
+/* Attention over the cache.  q [T, Hq, D], out the same (it may be q), Hq a multiple of Hk: head h reads the cache's head h / (Hq / Hk).  Rows starts[b] .. starts[b + 1] - 1 of q
+ * are the last tokens of request b, which has lengths[b] tokens in the cache, in the pages table[b] (M columns; starts [B + 1], lengths [B], table [B, M] i32); the one at
+ * position i sees tokens j <= i, with a window (not 0) i - window < j, whose page is in the table and in [0, pages).
+ *   out = sum over j of e^(z_j) v_j / sum of e^(z_j),  z_j = scale * q . k_j;  zeros for a row that sees none; rows of no request (before starts[0], behind starts[B])
+ * are not written, or zeros if `clear`.
+ * A row sees nothing of what others see alone: a NaN in a token's key or value reaches the rows that see it.  Scores, sums and statistics are held in 32 bits, e^z times a
+ * value's step in fp16 (2^-11 of it, and 2^-34 of the largest step so far among the tokens it sees), q as it is (but for 2^-35 of its largest element).
+ * longest: no request has more tokens than that (0: as many as the table has places for); the number of workgroups follows it, and results do not depend on it but for the order of sums.  */
+tts_status tts_kv4_attention_workspace(const tts_tensor *q, const tts_tensor *cache, const tts_tensor *table, int window, int64_t longest, size_t *bytes);
+tts_status tts_kv4_attention(const tts_tensor *q, const tts_tensor *cache, const tts_tensor *table, const tts_tensor *lengths, const tts_tensor *starts, double scale, int window,
+                             int64_t longest, int clear, const tts_tensor *out, void *workspace, size_t bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,13 @@ def lib():
     L.tts_moe_experts.argtypes = [t, t, t, t, t, t, t, flag, flag, t, *scratch, stream]
     L.tts_lora_add_workspace.argtypes = [t, t, size]
     L.tts_lora_add.argtypes = [t, t, t, t, t, t, t, *scratch, stream]
+    real, whole = ctypes.c_double, ctypes.c_int64
+    L.tts_page_slots.argtypes = [t, t, t, t, t, flag, t, t, t, t, t, stream]
+    L.tts_qk_norm_rope.argtypes = [t, t, t, t, t, t, real, flag, flag, t, t, stream]
+    L.tts_kv4_write.argtypes = [t, t, t, t, stream]
+    L.tts_kv4_read.argtypes = [t, t, t, t, stream]
+    L.tts_kv4_attention_workspace.argtypes = [t, t, t, flag, whole, size]
+    L.tts_kv4_attention.argtypes = [t, t, t, t, t, real, flag, whole, flag, t, *scratch, stream]
     _lib = L
     return L
 

@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <climits>
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/tts_hip.h"
@@ -177,6 +178,12 @@ struct Ops {
   decltype(&tts_moe_experts) experts;
   decltype(&tts_lora_add_workspace) lora_workspace;
   decltype(&tts_lora_add) lora;
+  decltype(&tts_page_slots) page_slots;
+  decltype(&tts_qk_norm_rope) rope;
+  decltype(&tts_kv4_write) kv4_write;
+  decltype(&tts_kv4_read) kv4_read;
+  decltype(&tts_kv4_attention_workspace) attend_workspace;
+  decltype(&tts_kv4_attention) attend;
   PyObject *get_device, *get_stream, *grad_enabled;  // torch._C._cuda_getDevice, _cuda_getCurrentRawStream, torch.is_grad_enabled
   PyObject *dtypes[5];                               // by tts_dtype
 };
@@ -246,7 +253,12 @@ struct Operands {
   // a new tensor on the device of `like`, [rows, cols] or (rows < 0) [cols], described; dtype null: of its type
   PyObject *make(PyObject *like, int64_t rows, int64_t cols, PyObject *dtype, tts_tensor &t) {
     if (!ok) return nullptr;
-    Ref size(rows < 0 ? Py_BuildValue("(L)", (long long)cols) : Py_BuildValue("(LL)", (long long)rows, (long long)cols));
+    return make(like, rows < 0 ? Py_BuildValue("(L)", (long long)cols) : Py_BuildValue("(LL)", (long long)rows, (long long)cols), dtype, t);
+  }
+  // the same of any shape, whose tuple it takes
+  PyObject *make(PyObject *like, PyObject *shape, PyObject *dtype, tts_tensor &t) {
+    Ref size(shape);
+    if (!ok) return nullptr;
     Ref names(dtype ? PyTuple_Pack(1, s_dtype) : nullptr);
     PyObject *args[] = {like, size.o, dtype};
     PyObject *made = size ? PyObject_VectorcallMethod(s_new_empty, args, 2, names.o) : nullptr;
@@ -340,12 +352,133 @@ PyObject *op_lora(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return finish(st, Py_NewRef(given ? a[6] : made.o));
 }
 
-// setup_ops(addresses of the five entries, torch._C._cuda_getDevice, _cuda_getCurrentRawStream, torch.is_grad_enabled, the five dtypes,
+// page_slots(table, lengths, fresh, free, count, page, rows)
+PyObject *op_page_slots(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 7) return not_ordinary();
+  Operands o(a[0]);
+  tts_tensor t[10];
+  int64_t page = 0, rows = 0;
+  if (!o.ok || !PyLong_CheckExact(a[5]) || !PyLong_CheckExact(a[6]) || !to_int64(a[5], &page) || !to_int64(a[6], &rows) || page < 1 || page > INT32_MAX || rows < 0 || rows > INT32_MAX)
+    return not_ordinary();
+  const tts_tensor *p[10] = {};
+  for (int i = 0; i < 5; i++) p[i] = o.describe(a[i], t[i]);
+  if (!o.ok || !p[0] || p[0]->rank != 2) return not_ordinary();
+  PyObject *result = PyTuple_New(5);
+  if (!result) return nullptr;
+  for (int i = 0; i < 5; i++) {
+    PyObject *made = o.make(a[0], -1, i < 3 ? rows : i == 3 ? t[0].shape[0] + 1 : 1, g_ops.dtypes[TTS_I32], t[5 + i]);
+    if (!o.ok) {
+      Py_XDECREF(made);
+      Py_DECREF(result);
+      return not_ordinary();
+    }
+    PyTuple_SET_ITEM(result, i, made);
+    p[5 + i] = &t[5 + i];
+  }
+  tts_status st;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_ops.page_slots(p[0], p[1], p[2], p[3], p[4], (int)page, p[5], p[6], p[7], p[8], p[9], o.stream);
+  Py_END_ALLOW_THREADS
+  return finish(st, result);
+}
+
+PyObject *shape_of(const tts_tensor &t) { return Py_BuildValue("(LLL)", (long long)t.shape[0], (long long)t.shape[1], (long long)t.shape[2]); }
+
+// qk_norm_rope(q, k, positions, cos_sin, w_q, w_k, eps, interleaved, q_out, k_out)
+PyObject *op_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 10) return not_ordinary();
+  Operands o(a[0]);
+  tts_tensor t[8];
+  if (!o.ok || !PyFloat_CheckExact(a[6]) || !PyBool_Check(a[7])) return not_ordinary();
+  const tts_tensor *p[8] = {};
+  for (int i = 0; i < 6; i++) p[i] = o.describe(a[i], t[i]);
+  const bool given = a[8] != Py_None;
+  if (given) p[6] = o.describe(a[8], t[6]), p[7] = o.describe(a[9], t[7]);
+  if (!o.ok || !p[0] || !p[1] || p[0]->rank != 3 || p[1]->rank != 3) return not_ordinary();
+  Ref q(given ? nullptr : o.make(a[0], shape_of(t[0]), nullptr, t[6])), k(given ? nullptr : o.make(a[1], shape_of(t[1]), nullptr, t[7]));
+  if (!o.ok) return not_ordinary();
+  if (!given) p[6] = &t[6], p[7] = &t[7];
+  const double eps = PyFloat_AS_DOUBLE(a[6]);
+  const bool interleaved = a[7] == Py_True;
+  tts_status st;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_ops.rope(p[0], p[1], p[2], p[3], p[4], p[5], eps, interleaved, !given, p[6], p[7], o.stream);
+  Py_END_ALLOW_THREADS
+  return finish(st, st == TTS_OK ? PyTuple_Pack(2, given ? a[8] : q.o, given ? a[9] : k.o) : nullptr);
+}
+
+// kv4_write(cache, k, v, slots)
+PyObject *op_kv4_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 4) return not_ordinary();
+  Operands o(a[0]);
+  tts_tensor t[4];
+  const tts_tensor *p[4] = {};
+  for (int i = 0; i < 4; i++) p[i] = o.describe(a[i], t[i]);
+  if (!o.ok) return not_ordinary();
+  tts_status st;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_ops.kv4_write(p[0], p[1], p[2], p[3], o.stream);
+  Py_END_ALLOW_THREADS
+  return finish(st, Py_NewRef(a[0]));
+}
+
+// kv4_read(cache, slots, dim)
+PyObject *op_kv4_read(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 3) return not_ordinary();
+  Operands o(a[0]);
+  tts_tensor t[4];
+  int64_t dim = 0;
+  if (!o.ok || !PyLong_CheckExact(a[2]) || !to_int64(a[2], &dim) || dim < 1 || dim > 256) return not_ordinary();
+  const tts_tensor *cache = o.describe(a[0], t[0]), *slots = o.describe(a[1], t[1]);
+  if (!o.ok || !cache || !slots || cache->rank != 3 || slots->rank != 1) return not_ordinary();
+  tts_tensor like = {};
+  like.shape[0] = t[1].shape[0], like.shape[1] = t[0].shape[1], like.shape[2] = dim;
+  Ref k(o.make(a[0], shape_of(like), nullptr, t[2])), v(o.make(a[0], shape_of(like), nullptr, t[3]));
+  if (!o.ok) return not_ordinary();
+  tts_status st;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_ops.kv4_read(cache, slots, &t[2], &t[3], o.stream);
+  Py_END_ALLOW_THREADS
+  return finish(st, st == TTS_OK ? PyTuple_Pack(2, k.o, v.o) : nullptr);
+}
+
+// kv4_attention(q, cache, table, lengths, starts, scale, window, longest, out): window and longest 0 for none
+PyObject *op_attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 9) return not_ordinary();
+  Operands o(a[0]);
+  tts_tensor t[6], scratch;
+  int64_t window = 0, longest = 0;
+  if (!o.ok || (a[5] != Py_None && !PyFloat_CheckExact(a[5])) || !PyLong_CheckExact(a[6]) || !PyLong_CheckExact(a[7]) || !to_int64(a[6], &window) || !to_int64(a[7], &longest) || window < 0 ||
+      window > INT32_MAX || longest < 0)
+    return not_ordinary();
+  const tts_tensor *p[6] = {};
+  for (int i = 0; i < 5; i++) p[i] = o.describe(a[i], t[i]);
+  if (!o.ok || !p[0] || !p[1] || !p[2] || p[0]->rank != 3 || p[0]->shape[2] < 1) return not_ordinary();
+  size_t bytes = 0;
+  tts_status st = g_ops.attend_workspace(p[0], p[1], p[2], (int)window, longest, &bytes);
+  if (st != TTS_OK) return finish(st, nullptr);
+  const bool given = a[8] != Py_None;
+  if (given) p[5] = o.describe(a[8], t[5]);
+  Ref made(given ? nullptr : o.make(a[0], shape_of(t[0]), nullptr, t[5]));
+  Ref work(bytes ? o.make(a[0], -1, (int64_t)bytes, g_ops.dtypes[TTS_I8], scratch) : nullptr);
+  if (!o.ok) return not_ordinary();
+  p[5] = &t[5];
+  void *at = bytes ? scratch.ptr : nullptr;
+  const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)t[0].shape[2]) : PyFloat_AS_DOUBLE(a[5]);
+  Py_BEGIN_ALLOW_THREADS
+  st = g_ops.attend(p[0], p[1], p[2], p[3], p[4], scale, (int)window, longest, !given, p[5], at, bytes, o.stream);
+  Py_END_ALLOW_THREADS
+  return finish(st, Py_NewRef(given ? a[8] : made.o));
+}
+
+// setup_ops(addresses of the eleven entries, torch._C._cuda_getDevice, _cuda_getCurrentRawStream, torch.is_grad_enabled, the five dtypes,
 // torch.Tensor, torch.nn.Parameter, _raise)
 PyObject *setup_ops(PyObject *, PyObject *args) {
-  unsigned long long f[5];
+  unsigned long long f[11];
   PyObject *o[11];
-  if (!PyArg_ParseTuple(args, "KKKKKOOOOOOOOOOO", &f[0], &f[1], &f[2], &f[3], &f[4], &o[0], &o[1], &o[2], &o[3], &o[4], &o[5], &o[6], &o[7], &o[8], &o[9], &o[10])) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKOOOOOOOOOOO", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7], &f[8], &f[9], &f[10], &o[0], &o[1], &o[2], &o[3], &o[4], &o[5], &o[6], &o[7],
+                        &o[8], &o[9], &o[10]))
+    return nullptr;
   PyObject **to[11] = {&g_ops.get_device, &g_ops.get_stream, &g_ops.grad_enabled, &g_ops.dtypes[0], &g_ops.dtypes[1], &g_ops.dtypes[2], &g_ops.dtypes[3], &g_ops.dtypes[4], &g_tensor_type,
                        &g_parameter_type, &g_raise};
   for (int i = 0; i < 11; i++) {
@@ -356,6 +489,12 @@ PyObject *setup_ops(PyObject *, PyObject *args) {
   g_ops.experts = (decltype(g_ops.experts))(uintptr_t)f[2];
   g_ops.lora_workspace = (decltype(g_ops.lora_workspace))(uintptr_t)f[3];
   g_ops.lora = (decltype(g_ops.lora))(uintptr_t)f[4];
+  g_ops.page_slots = (decltype(g_ops.page_slots))(uintptr_t)f[5];
+  g_ops.rope = (decltype(g_ops.rope))(uintptr_t)f[6];
+  g_ops.kv4_write = (decltype(g_ops.kv4_write))(uintptr_t)f[7];
+  g_ops.kv4_read = (decltype(g_ops.kv4_read))(uintptr_t)f[8];
+  g_ops.attend_workspace = (decltype(g_ops.attend_workspace))(uintptr_t)f[9];
+  g_ops.attend = (decltype(g_ops.attend))(uintptr_t)f[10];
   g_ops.route = (decltype(g_ops.route))(uintptr_t)f[0];
   Py_RETURN_NONE;
 }
@@ -365,6 +504,11 @@ PyMethodDef module_methods[] = {{"setup", setup, METH_VARARGS, nullptr},
                                 {"moe_route", (PyCFunction)(void (*)(void))op_route, METH_FASTCALL, nullptr},
                                 {"moe_experts", (PyCFunction)(void (*)(void))op_experts, METH_FASTCALL, nullptr},
                                 {"lora_add", (PyCFunction)(void (*)(void))op_lora, METH_FASTCALL, nullptr},
+                                {"page_slots", (PyCFunction)(void (*)(void))op_page_slots, METH_FASTCALL, nullptr},
+                                {"qk_norm_rope", (PyCFunction)(void (*)(void))op_rope, METH_FASTCALL, nullptr},
+                                {"kv4_write", (PyCFunction)(void (*)(void))op_kv4_write, METH_FASTCALL, nullptr},
+                                {"kv4_read", (PyCFunction)(void (*)(void))op_kv4_read, METH_FASTCALL, nullptr},
+                                {"kv4_attention", (PyCFunction)(void (*)(void))op_attend, METH_FASTCALL, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "tts_launch", nullptr, -1, module_methods, nullptr, nullptr, nullptr, nullptr};
 

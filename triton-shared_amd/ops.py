@@ -1,15 +1,25 @@
-"""Operators whose weights are picked per row of activations: what a decode step does beside its shared projections.
+"""Operators of a decode step beside its shared projections.  Those whose weights are picked per row of activations:
 
     ids, weights = ops.moe_route(logits, 8)                                  # the router, from its logits
     y = ops.moe_experts(x, ids, weights, w_up, w_down)                       # the experts of a few tokens
     q = ops.lora_add(q, x, a, b, adapter_of_row, scales=scales, out=q)       # adapters of many requests, after the projection
 
-They are hand-written kernels behind the C ABI (include/tts_hip.h: tts_moe_route, tts_moe_experts, tts_lora_add), for code that
-calls them beside its Triton kernels: on the current stream of their tensors' device, asynchronous, capturable into a graph.
+and its attention over a paged cache held in 4 bits:
+
+    cache = ops.kv4_cache(pages, kv_heads, dim, page=16)                                                       # once, of each layer
+    slots, positions, owners, starts, left = ops.page_slots(table, lengths, fresh, free, count, 16, rows)      # once a step, for all layers
+    q, k = ops.qk_norm_rope(q, k, positions, cos_sin, w_q, w_k)
+    ops.kv4_write(cache, k, v, slots)
+    y = ops.kv4_attention(q, cache, table, lengths, starts)                                                    # (kv4_read: what slots hold, as values)
+
+They are hand-written kernels behind the C ABI (include/tts_hip.h: tts_moe_route, tts_moe_experts, tts_lora_add, tts_page_slots, tts_qk_norm_rope,
+tts_kv4_write, tts_kv4_read, tts_kv4_attention), for code that calls them beside its Triton kernels: on the current stream of their tensors' device,
+asynchronous, capturable into a graph.
 Wrong arguments raise ValueError or TypeError, what is not implemented NotImplementedError, failing HIP calls RuntimeError.
 They have no derivatives: tensors that require gradients are refused where gradients are recorded, and those with a forward-mode tangent anywhere.
 """
 import ctypes
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -47,15 +57,17 @@ _fast = None
 
 
 def _native_calls():
-    """The launch extension's own moe_route, moe_experts and lora_add (csrc/launch_module.cpp), which take the ordinary calls; False without it."""
+    """The launch extension's functions of the names below (csrc/launch_module.cpp), which take the ordinary calls; False without it."""
     global _fast
     module, lib = _native.launch_module(), _native.lib()
     if module is None:
         _fast = False
     else:
         address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
-        module.setup_ops(address(lib.tts_moe_route), address(lib.tts_moe_experts_workspace), address(lib.tts_moe_experts), address(lib.tts_lora_add_workspace), address(lib.tts_lora_add),
-                         torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, *_DTYPES, torch.Tensor, torch.nn.Parameter, _native._raise)
+        entries = (lib.tts_moe_route, lib.tts_moe_experts_workspace, lib.tts_moe_experts, lib.tts_lora_add_workspace, lib.tts_lora_add, lib.tts_page_slots, lib.tts_qk_norm_rope,
+                   lib.tts_kv4_write, lib.tts_kv4_read, lib.tts_kv4_attention_workspace, lib.tts_kv4_attention)
+        module.setup_ops(*map(address, entries), torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, *_DTYPES, torch.Tensor, torch.nn.Parameter,
+                         _native._raise)
         _fast = module
     return _fast
 
@@ -84,6 +96,14 @@ def _written(out):
     """`out`, of which autograd knows now that it has changed: a backward pass that has saved it raises."""
     torch.autograd.graph.increment_version(out)
     return out
+
+
+def _whole(name, value):
+    """An integer argument, which C's conversion would cut to 32 bits."""
+    value = operator.index(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{name} is {value}")
+    return value
 
 
 def _call(entry, device, *args):
@@ -171,4 +191,133 @@ def lora_add(base, x, a, b, ids, scales=None, out=None):
     given, out = out, torch.empty_like(base, memory_format=torch.contiguous_format) if out is None else out
     _call(_native.lib().tts_lora_add, device, db, dx, da, dl, _describe("ids", ids, device), _describe("scales", scales, device), _describe("out", out, device), work.data_ptr(),
           work.numel())
+    return out if given is None else _written(out)
+
+
+def page_slots(table, lengths, fresh, free, count, page, rows):
+    """Block tables and slot maps of a step, from its requests' lengths: (slots [rows], positions [rows], owners [rows], starts [B + 1], left [1]), all int32.
+
+    table [B, M] int32 holds the pages of each request in order (`page` tokens each); lengths [B] int32 the tokens it has after this step, fresh [B] int32 how many of them are new, its last ones.
+    free [F] int32 is a stack of free pages, the first count[0] of it, the last of them the top.  Requests take the pages that they lack from the top, the first
+    request first, and those are written into `table` (-1 where the stack has run out); `left` is what count is afterwards.  The step's rows are the new tokens of one request after another:
+    request b's are starts[b] .. starts[b + 1] - 1, `owners` has the request of each, `positions` its position and `slots` its place in the cache, for `kv4_write`.  A row
+    without a page has slot -1, and rows behind the last request's -1 in all three.  B up to 4096.
+    """
+    fast = _ordinary()
+    if fast:
+        made = fast.page_slots(table, lengths, fresh, free, count, page, rows)
+        if made is not None:
+            _written(table)
+            return made
+    device = _device_of("table", table)
+    if table.dim() != 2:
+        raise ValueError(f"table has {table.dim()} dimensions, not 2")
+    page, rows = _whole("page", page), _whole("rows", rows)
+    if rows < 0:
+        raise ValueError(f"rows is {rows}")
+    sizes = (rows, rows, rows, table.shape[0] + 1, 1)
+    made = tuple(torch.empty(n, dtype=torch.int32, device=device) for n in sizes)
+    _call(_native.lib().tts_page_slots, device, *(_describe(n, t, device) for n, t in (("table", table), ("lengths", lengths), ("fresh", fresh), ("free", free), ("count", count))), page,
+          *(_describe(n, t, device) for n, t in zip(("slots", "positions", "owners", "starts", "left"), made)))
+    _written(table)
+    return made
+
+
+def qk_norm_rope(q, k, positions, cos_sin, w_q=None, w_k=None, eps=1e-6, interleaved=False, out=None):
+    """Norms of queries and keys for each head, and the rotation by position, in one pass: (q, k) turned.
+
+    q [T, Hq, D] and k [T, Hk, D] in float32, float16 or bfloat16 (D even, up to 512), views of one projection's rows as well.  Of each head y = x / sqrt(mean(x^2) + eps) * w, with w_q and
+    w_k [D] of its type or float32 (without them y = x); then pairs (a, b) of its first R elements become (a cos - b sin, b cos + a sin): elements n and n + R / 2, or 2 n and
+    2 n + 1 if `interleaved`.  cos_sin [P, R] float32 has the cosines of a position's R / 2 angles, then their sines; positions [T] int32.  Rows whose position is not in [0, P) are padding:
+    zeros in what is returned, or, in an `out` that is given, as they were.  `out` is a pair (q, k) and may be q and k themselves.
+    """
+    fast = _ordinary()
+    given = out is not None
+    q_out, k_out = out if given else (None, None)
+    if given and (q_out is None or k_out is None):
+        raise ValueError("out is a pair of tensors")
+    if fast:
+        made = fast.qk_norm_rope(q, k, positions, cos_sin, w_q, w_k, eps, interleaved, q_out, k_out)
+        if made is not None:
+            return (_written(q_out), _written(k_out)) if given else made
+    device = _device_of("q", q)
+    dq, dk = _describe("q", q, device), _describe("k", k, device)
+    if not given:
+        q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
+    _call(_native.lib().tts_qk_norm_rope, device, dq, dk, _describe("positions", positions, device), _describe("cos_sin", cos_sin, device), _describe("w_q", w_q, device),
+          _describe("w_k", w_k, device), float(eps), bool(interleaved), not given, _describe("q_out", q_out, device), _describe("k_out", k_out, device))
+    return (_written(q_out), _written(k_out)) if given else (q_out, k_out)
+
+
+def kv4_cache(pages, heads, dim, page=16, dtype=torch.bfloat16, device="cuda"):
+    """An empty cache of 4 bits for one layer: [pages, heads, page * (dim + 8) / 2] of `dtype` (float16 or bfloat16, the type of its keys and values), whose inner layout the operators know.
+
+    `dim` is a multiple of 32 up to 256, `page` (the tokens of a page) a multiple of 16.  What it takes is dim + 8 bytes for a token's key and value of each head.
+    """
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"dtype is {dtype}, not float16 or bfloat16")
+    if dim % 32 or not 32 <= dim <= 256:
+        raise NotImplementedError(f"heads of {dim} elements, not a multiple of 32 up to 256")
+    if page % 16 or page < 16:
+        raise NotImplementedError(f"pages of {page} tokens, not a multiple of 16")
+    return torch.zeros(pages, heads, page * (dim + 8) // 2, dtype=dtype, device=device)
+
+
+def kv4_write(cache, k, v, slots):
+    """Puts keys and values k, v [T, Hk, D] of the cache's type into its slots [T] int32 and returns the cache; rows whose slot is not in it (-1: padding) are left out.
+
+    Of each head of a token, and of key and value each: an element x is held as code * step + lowest, step = (highest - lowest) / 15 rounded to the type, code the number of borders (n + 1/2) * step
+    that x - lowest is above.  What is not finite makes the head NaN.  The slots in the cache are distinct (as `page_slots` gives them).
+    """
+    fast = _ordinary()
+    if fast and fast.kv4_write(cache, k, v, slots) is not None:
+        return _written(cache)
+    device = _device_of("cache", cache)
+    _call(_native.lib().tts_kv4_write, device, _describe("cache", cache, device), _describe("k", k, device), _describe("v", v, device), _describe("slots", slots, device))
+    return _written(cache)
+
+
+def kv4_read(cache, slots, dim):
+    """The keys and values [T, Hk, dim] that slots [T] int32 of a cache hold, as values of its type; zeros for a slot that is not in it."""
+    fast = _ordinary()
+    if fast:
+        made = fast.kv4_read(cache, slots, dim)
+        if made is not None:
+            return made
+    device = _device_of("cache", cache)
+    if cache.dim() != 3:
+        raise ValueError(f"cache has {cache.dim()} dimensions, not 3")
+    ds = _describe("slots", slots, device)
+    if slots.dim() != 1:
+        raise ValueError(f"slots have {slots.dim()} dimensions, not 1")
+    k, v = (torch.empty(slots.shape[0], cache.shape[1], _whole("dim", dim), dtype=cache.dtype, device=device) for _ in range(2))
+    _call(_native.lib().tts_kv4_read, device, _describe("cache", cache, device), ds, _describe("k", k, device), _describe("v", v, device))
+    return k, v
+
+
+def kv4_attention(q, cache, table, lengths, starts, scale=None, window=None, longest=None, out=None):
+    """Attention of a step's rows over the cache:
+
+        out[t, h] = sum over j of softmax_j(scale * q[t, h] . k_j) v_j
+
+    q [T, Hq, D] of the cache's type, Hq a multiple of its heads: head h reads the cache's head h // (Hq // Hk).  Rows starts[b] .. starts[b + 1] - 1 are the last tokens of request b, which has
+    lengths[b] tokens in the pages table[b] (table [B, M], lengths [B], starts [B + 1], all int32, as `page_slots` leaves them); the row at position i sees the tokens j <= i, with a
+    `window` those of i - window < j.  scale is D ** -0.5 unless it is given.  A row that sees nothing is zeros; rows of no request are zeros too, or as they were in an `out` that is given (it may be q).
+    `longest`, a length that no request passes, lets short requests in a wide table do with fewer workgroups.
+    """
+    if window is not None and _whole("window", window) < 1:
+        raise ValueError(f"window is {window}")
+    if longest is not None and _whole("longest", longest) < 1:
+        raise ValueError(f"longest is {longest}")
+    fast = _ordinary()
+    if fast:
+        made = fast.kv4_attention(q, cache, table, lengths, starts, scale, window or 0, longest or 0, out)
+        if made is not None:
+            return made if out is None else _written(out)
+    device = _device_of("q", q)
+    dq, dc, dt = _describe("q", q, device), _describe("cache", cache, device), _describe("table", table, device)
+    work = _workspace(_native.lib().tts_kv4_attention_workspace, device, dq, dc, dt, window or 0, longest or 0)
+    given, out = out, torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    _call(_native.lib().tts_kv4_attention, device, dq, dc, dt, _describe("lengths", lengths, device), _describe("starts", starts, device), float(q.shape[2] ** -0.5 if scale is None else scale),
+          window or 0, longest or 0, given is None, _describe("out", out, device), work.data_ptr(), work.numel())
     return out if given is None else _written(out)
