@@ -7,6 +7,19 @@
 
 namespace tts {
 
+// n / divisor for 0 <= n < 2^31 is n * mul >> shift
+struct FastDiv {
+  uint32_t mul;
+  int shift;
+};
+inline FastDiv fast_div(uint32_t divisor) {
+  int up = 0;
+  while (((uint64_t)1 << up) < divisor) up++;
+  return {(uint32_t)((((uint64_t)1 << (31 + up)) + divisor - 1) / divisor), 31 + up};
+}
+
+__device__ __forceinline__ int divided(int n, FastDiv by) { return (int)(((uint64_t)(uint32_t)n * by.mul) >> by.shift); }
+
 constexpr int SLOTS_MAX_REQUESTS = 4096;
 
 struct SlotsParams {
@@ -35,6 +48,7 @@ struct RopeParams {
   float eps;
   int elem;             // ElemKind of q and k
   int w_f32, interleaved, clear;
+  FastDiv by_chunks;    // of a token's heads (the launch's own)
 };
 hipError_t launch_rope(const RopeParams &p, hipStream_t s);
 
@@ -48,6 +62,7 @@ struct Kv4Cache {
   void *base;
   int64_t page_bytes, head_bytes;  // from page to page, from head to head
   int pages, heads, page, dim, bf16;
+  FastDiv by_page;
 };
 
 struct Kv4RowsParams {
@@ -55,17 +70,19 @@ struct Kv4RowsParams {
   void *k, *v;          // [tokens, heads, dim]
   const int *slots;     // [tokens]
   int64_t k_token, k_head, v_token, v_head, tokens;
+  FastDiv by_heads;     // of keys and of values (the launch's own)
 };
 hipError_t launch_kv4_write(const Kv4RowsParams &p, hipStream_t s);
 hipError_t launch_kv4_read(const Kv4RowsParams &p, hipStream_t s);
 
 // How a call's rows and lengths are dealt to workgroups (kernels_kv4_attend.hip)
 struct AttendPlan {
-  int row_tiles;        // of 16 rows, that a wavefront holds
   int by_rows;          // the four wavefronts have rows of their own (else a share of the tokens each)
-  int tile;             // rows of a workgroup
-  int64_t items;        // workgroups per head of the cache and slice, at most
-  int slices, slice;    // at most, and the tokens of each
+  int tile_log;         // log2 of a workgroup's rows
+  int64_t items;        // tiles of rows per head of the cache, at most
+  int64_t extra;        // workgroups beyond one for each of them: slices of their tokens (0: none are sliced)
+  float over_extra;     // 1 / extra
+  int round;            // a slice has a multiple of so many blocks of 64 tokens
 };
 
 struct AttendParams {
@@ -76,16 +93,18 @@ struct AttendParams {
   const int *lengths;   // [requests]
   const int *starts;    // [requests + 1]
   int64_t q_token, q_head, o_token, o_head, ld_table, tokens;
-  int requests, columns, heads, group;
+  int requests, heads, group;
+  int places;           // tokens that a request's row of the table has places for
+  FastDiv by_group, by_heads, by_kv_heads;
   int window;           // 0: none
   int clear;            // rows of no request get zeros
   float scale;
   AttendPlan plan;
-  float *parts;         // [tokens * heads, slices, dim]
-  float *stats;         // [tokens * heads, slices, 2]
+  float *parts;         // [workgroups, tile, dim] of what is sliced
+  float *stats;         // [workgroups, tile, 2]
 };
 AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, int dim, int64_t longest, int window);
-size_t attend_workspace_bytes(const AttendPlan &plan, int64_t tokens, int heads, int dim);
+size_t attend_workspace_bytes(const AttendPlan &plan, int kv_heads, int dim);
 hipError_t launch_attend(const AttendParams &p, hipStream_t s);
 
 }  // namespace tts

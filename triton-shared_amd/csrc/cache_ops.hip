@@ -2,6 +2,7 @@
 // checked here, on the host, before anything is launched.
 #include "cache_ops.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -26,7 +27,7 @@ Kv4Cache cache_of(const Arg &a, int64_t dim) {
   a.present();
   Kv4Cache c = {};
   c.base = a.t->ptr, c.page_bytes = a.stride(0) * 2, c.head_bytes = a.stride(1) * 2;
-  c.pages = (int)a.size(0), c.heads = (int)a.size(1), c.page = (int)page, c.dim = (int)dim, c.bf16 = a.t->dtype == TTS_BF16;
+  c.pages = (int)a.size(0), c.heads = (int)a.size(1), c.page = (int)page, c.dim = (int)dim, c.bf16 = a.t->dtype == TTS_BF16, c.by_page = fast_div((uint32_t)page);
   return c;
 }
 
@@ -57,17 +58,19 @@ struct Attend {
     p.cache = cache_of(cache, q.size(2));
     q.type(cache.t->dtype);
     table.rank(2).type(TTS_I32).neighbours();
-    p.tokens = q.size(0), p.heads = (int)q.size(1), p.requests = (int)table.size(0), p.columns = (int)table.size(1), p.window = window;
+    p.tokens = q.size(0), p.heads = (int)q.size(1), p.requests = (int)table.size(0), p.window = window;
     if (p.heads < 1 || p.heads % p.cache.heads) invalid("q: " + std::to_string(p.heads) + " heads, not a multiple of the cache's " + std::to_string(p.cache.heads));
     p.group = p.heads / p.cache.heads;
     if (window < 0) invalid("the window is " + std::to_string(window));
     if (longest < 0) invalid("longest is " + std::to_string(longest));
     if (p.tokens * p.heads > ((int64_t)1 << 26)) unsupported("q: " + std::to_string(p.tokens) + " rows of " + std::to_string(p.heads) + " heads");
     if (p.requests > (1 << 20)) unsupported("table: " + std::to_string(p.requests) + " requests");
-    const int64_t most = std::min((int64_t)p.columns * p.cache.page, (int64_t)INT_MAX / 2);
+    const int64_t most = std::min(table.size(1) * p.cache.page, (int64_t)INT_MAX / 2);
+    p.places = (int)most;
+    p.by_group = fast_div(p.group), p.by_heads = fast_div(p.heads), p.by_kv_heads = fast_div(p.cache.heads);
     p.plan = plan_attend(p.tokens, p.requests, p.heads, p.cache.heads, p.cache.dim, longest ? std::min(longest, most) : most, window);
     // (a launch of 2^32 lanes and more starts only their remainder)
-    if (p.plan.items * p.cache.heads * p.plan.slices >= (1 << 24)) unsupported(std::to_string(p.requests) + " requests of " + std::to_string(p.cache.heads) + " heads: more workgroups than a launch has");
+    if ((p.plan.items + p.plan.extra) * p.cache.heads >= (1 << 24)) unsupported(std::to_string(p.requests) + " requests of " + std::to_string(p.cache.heads) + " heads: more workgroups than a launch has");
   }
 };
 
@@ -178,7 +181,7 @@ tts_status tts_kv4_attention_workspace(const tts_tensor *q, const tts_tensor *ca
   return guarded("tts_kv4_attention_workspace", [&]() -> hipError_t {
     if (!bytes) invalid("bytes is missing");
     const Attend a(q, cache, table, window, longest);
-    *bytes = attend_workspace_bytes(a.p.plan, a.p.tokens, a.p.heads, a.p.cache.dim);
+    *bytes = attend_workspace_bytes(a.p.plan, a.p.cache.heads, a.p.cache.dim);
     return hipSuccess;
   });
 }
@@ -196,13 +199,13 @@ tts_status tts_kv4_attention(const tts_tensor *q_, const tts_tensor *cache_, con
     for (const Arg *x : {&a.q, &a.table, &lengths, &starts, &out}) x->present();
     same_or_apart(out, a.q);
     apart(out, a.cache), apart(out, a.table), apart(out, lengths), apart(out, starts);
-    const size_t need = attend_workspace_bytes(p.plan, p.tokens, p.heads, p.cache.dim);
+    const size_t need = attend_workspace_bytes(p.plan, p.cache.heads, p.cache.dim);
     check_workspace(workspace, bytes, need);
     if (!p.tokens || (!p.requests && !clear)) return hipSuccess;
     p.q = a.q.t->ptr, p.out = out.t->ptr, p.table = (const int *)a.table.t->ptr, p.lengths = (const int *)lengths.t->ptr, p.starts = (const int *)starts.t->ptr;
     p.q_token = a.q.stride(0), p.q_head = a.q.stride(1), p.o_token = out.stride(0), p.o_head = out.stride(1), p.ld_table = a.table.stride(0);
     p.scale = (float)scale, p.clear = clear != 0;
-    p.parts = (float *)workspace, p.stats = p.parts + p.tokens * p.heads * p.plan.slices * p.cache.dim;
+    p.parts = (float *)workspace, p.stats = p.parts + ((p.plan.items + p.plan.extra) * p.cache.heads << p.plan.tile_log) * p.cache.dim;
     return launch_attend(p, (hipStream_t)stream);
   });
 }

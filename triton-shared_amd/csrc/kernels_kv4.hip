@@ -23,7 +23,7 @@ struct Place {
 };
 // where a slot's head is (`values`: its value, else its key)
 __device__ __forceinline__ Place place_of(const Kv4Cache &c, int slot, int head, int values) {
-  const int page = slot / c.page, at = slot % c.page;
+  const int page = divided(slot, c.by_page), at = slot - page * c.page;
   char *base = (char *)c.base + page * c.page_bytes + head * c.head_bytes;
   return {base + ((int64_t)values * c.page + at) * (c.dim / 2), base + (int64_t)c.page * c.dim + ((int64_t)values * c.page + at) * 4};
 }
@@ -36,14 +36,13 @@ template <class T, int L>
 __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4RowsParams p) {
   const Kv4Cache &c = p.cache;
   const int lane = threadIdx.x % L;
-  const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int64_t t = item / (2 * c.heads);
+  const int item = blockIdx.x * (256 / L) + threadIdx.x / L, t = divided(item, p.by_heads);
   if (t >= p.tokens) return;
-  const int rest = (int)(item % (2 * c.heads)), values = rest >= c.heads, head = values ? rest - c.heads : rest;
+  const int rest = item - t * 2 * c.heads, values = rest >= c.heads, head = values ? rest - c.heads : rest;
   const int slot = p.slots[t];
   if (slot < 0 || slot >= c.pages * c.page) return;
   const bool mine = lane * 8 < c.dim;
-  const T *row = (const T *)(values ? p.v : p.k) + t * (values ? p.v_token : p.k_token) + head * (values ? p.v_head : p.k_head);
+  const T *row = (const T *)(values ? p.v : p.k) + (int64_t)t * (values ? p.v_token : p.k_token) + head * (values ? p.v_head : p.k_head);
   T x[8];
   __builtin_memcpy(x, row + (mine ? lane * 8 : 0), sizeof x);
   float low = (float)x[0], high = low;
@@ -61,19 +60,30 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4RowsParams p) {
   const float step = (float)step_t;
   finite &= range < __builtin_inff();
   u32 word = 0;
-  if (finite && step > 0.f)
+  if (finite && step > 0.f) {
+    // The border next to x - lowest, as 32 bits have it, decides between the codes on its sides: that comparison is exact, since borders are whole in 32 bits, but where both
+    // are the same there, when what 32 bits leave of the difference decides (seldom: off the way of the others)
+    const int power = __builtin_amdgcn_frexp_expf(step);
+    const float over = 1.f / __builtin_amdgcn_ldexpf(step, -power);
+    float d[8], border[8], code[8];
+    bool even = false;
     for (int e = 0; e < 8; e++) {
-      // x - lowest is d + rest, without an error; borders are whole in 32 bits
-      const float v = (float)x[e], d = v - low, back = v - d, rest = (v - (d + back)) + (back - low);
-      auto above = [&](int n) __attribute__((always_inline)) {
-        const float border = ((float)n + 0.5f) * step;
-        return d > border || (d == border && rest > 0.f);
-      };
-      int code = (int)fminf(fmaxf(ceilf(d / step - 0.5f), 0.f), 15.f);
-      if (code > 0 && !above(code - 1)) code--;
-      else if (code < 15 && above(code)) code++;
-      word |= (u32)code << (values ? shift_of(e, true) : shift_of(e, false));
+      d[e] = (float)x[e] - low;
+      border[e] = __builtin_amdgcn_fmed3f(__builtin_rintf(__builtin_fmaf(__builtin_amdgcn_ldexpf(d[e], -power), over, -0.5f)), 0.f, 14.f);
+      const float at = (border[e] + 0.5f) * step;
+      code[e] = d[e] > at ? border[e] + 1.f : border[e];
+      even |= d[e] == at;
     }
+    if (__any(even))
+      for (int e = 0; e < 8; e++) {
+        const float v = (float)x[e], back = v - d[e], rest = (v - (d[e] + back)) + (back - low);  // x - lowest is d + rest, without an error
+        if (d[e] == (border[e] + 0.5f) * step && rest > 0.f) code[e] = border[e] + 1.f;
+      }
+    // (the codes by twos in 32 bits; exact)
+    u32 two[4];
+    for (int e = 0; e < 4; e++) two[e] = (u32)__builtin_fmaf(code[2 * e + 1], values ? 16.f : 65536.f, code[2 * e]);
+    word = values ? two[0] | two[1] << 8 | two[2] << 16 | two[3] << 24 : two[0] | two[1] << 4 | two[2] << 8 | two[3] << 12;
+  }
   const Place at = place_of(c, slot, head, values);
   if (mine) *(u32 *)(at.codes + lane * 4) = word;
   if (lane == 0) *(u32 *)at.pair = finite ? bits_of(step_t) | bits_of((T)(low + 0.f)) << 16 : bits_of((T)__builtin_nanf(""));
@@ -84,12 +94,11 @@ template <class T, int L>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsParams p) {
   const Kv4Cache &c = p.cache;
   const int lane = threadIdx.x % L;
-  const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int64_t t = item / (2 * c.heads);
+  const int item = blockIdx.x * (256 / L) + threadIdx.x / L, t = divided(item, p.by_heads);
   if (t >= p.tokens || lane * 8 >= c.dim) return;
-  const int rest = (int)(item % (2 * c.heads)), values = rest >= c.heads, head = values ? rest - c.heads : rest;
+  const int rest = item - t * 2 * c.heads, values = rest >= c.heads, head = values ? rest - c.heads : rest;
   const int slot = p.slots[t];
-  T *row = (T *)(values ? p.v : p.k) + t * (values ? p.v_token : p.k_token) + head * (values ? p.v_head : p.k_head);
+  T *row = (T *)(values ? p.v : p.k) + (int64_t)t * (values ? p.v_token : p.k_token) + head * (values ? p.v_head : p.k_head);
   T x[8] = {};
   if (slot >= 0 && slot < c.pages * c.page) {
     const Place at = place_of(c, slot, head, values);
@@ -102,9 +111,10 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsParams p) {
 
 template <class T, class K>
 hipError_t go(const Kv4RowsParams &p, int lanes, hipStream_t s, K kernel) {
-  const int64_t per = 256 / lanes, heads = 2 * p.cache.heads, each = ((int64_t)1 << 22) * per / heads;  // tokens of a launch (less than 2^32 lanes)
+  const int64_t per = 256 / lanes, heads = 2 * p.cache.heads, each = ((int64_t)1 << 22) * per / heads;  // tokens of a launch (less than 2^32 lanes, and than 2^31 heads)
   for (int64_t at = 0; at < p.tokens; at += each) {
     Kv4RowsParams part = p;
+    part.by_heads = fast_div((uint32_t)heads);
     part.tokens = std::min(each, p.tokens - at);
     part.slots += at;
     part.k = (T *)p.k + at * p.k_token, part.v = (T *)p.v + at * p.v_token;

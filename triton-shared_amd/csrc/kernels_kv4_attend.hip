@@ -12,8 +12,10 @@
 // left operand of  scores[token][row];  so a lane gets the scores of tokens 4 g .. 4 g + 3 of each tile for row m, and what it makes of them is the right
 // operand of  out[element][row]  as it stands.  Its left operand, 16 tokens of one element per lane, is read out of LDS by ds_read_b64_tr_b4.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_ops.h"
+#include "lanes.h"
 #include "row_device.h"
 
 namespace tts {
@@ -28,15 +30,20 @@ using row_ops::mfma16;
 using row_ops::u32;
 
 constexpr int WAVES = 4, BLOCK = 64;  // tokens
+constexpr int MOST_SLICES = 128;
 constexpr float LOG2_E = 1.4426950408889634f;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
-// f over the four lanes of a row (those 16 apart)
-template <class F>
+// f over the lanes of a row: those 16 apart by exchanges of 16 and of 32 lanes in registers, and those ROWS apart in 16 lanes
+template <int ROWS = 16, class F>
 __device__ __forceinline__ float over_row(float v, F f) {
-  v = f(v, __shfl_xor(v, 16));
-  return f(v, __shfl_xor(v, 32));
+  if constexpr (ROWS <= 4) v = f(v, dpp_moved<0x124>(v));  // row_ror 4
+  if constexpr (ROWS <= 8) v = f(v, dpp_moved<0x128>(v));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // a word's codes as four pairs, in the order of its bits 0 and 16, 4 and 20, 8 and 24, 12 and 28; the second and the last 2^4 as much
@@ -52,231 +59,345 @@ __device__ __forceinline__ u32 fp16_pair(float a, float b) {
   return __builtin_bit_cast(u32, v);
 }
 
-// The request and the rows of it that a workgroup has; what follows of them for tokens.
-struct Rows {
-  int request, first, rows;       // of the step's rows: where the request's begin, and how many it has
-  int length, tokens;             // of the request, and how many of them the table can hold
-  int begin, end;                 // what the tile's rows see lies in [begin, end), begin at a multiple of 16
-  int slices;
+// What a call's workgroups (of one head of the cache) do: each request's tiles of rows, one after another, and of each its slices of the tokens that the request's
+// rows see.  Slices are of one length for all requests, so that a batch of ragged lengths makes workgroups of one size: their number is what the call has beyond one for each
+// tile, and their length what it takes to deal all tokens to that many.  Every wavefront works that out for itself, a request per lane.
+struct Work {
+  int request, first, rows;     // of the step's rows: where the request's begin, and how many it has (0: nothing to do)
+  int tile, slice, slices;
+  int length, tokens;           // of the request, and how many of them the table can hold
+  int begin, size;              // the first token that its rows see, at a multiple of 16, and a slice's tokens
+  int index;                    // of its first workgroup
 };
 
 // (starts are the caller's memory: whatever they hold, rows stay inside [0, tokens))
 __device__ __forceinline__ int start_of(const AttendParams &p, int b) { return (int)min((int64_t)max(p.starts[b], 0), p.tokens); }
 
-__device__ __forceinline__ Rows rows_of(const AttendParams &p, int b, int tile) {
-  Rows r;
-  r.request = b, r.first = start_of(p, b), r.rows = max(start_of(p, b + 1) - r.first, 0);
-  r.length = max(p.lengths[b], 0);
-  r.tokens = (int)min((int64_t)r.length, (int64_t)p.columns * p.cache.page);
-  const int top = tile * p.plan.tile / p.group, bottom = min((tile * p.plan.tile + p.plan.tile - 1) / p.group, r.rows - 1);
-  const int behind = r.length - r.rows + 1;  // what row 0 sees ends there
-  r.begin = p.window ? max(behind + top - p.window, 0) / 16 * 16 : 0;
-  r.end = min(behind + bottom, r.tokens);
-  const int slices = (r.end - r.begin + p.plan.slice - 1) / p.plan.slice;
-  r.slices = min(max(slices, 1), p.plan.slices);
+struct Request {
+  int first, rows, length, tokens, begin, blocks, tiles;  // blocks: of 64 tokens, of what its rows see
+};
+__device__ __forceinline__ Request request_of(const AttendParams &p, int b) {
+  Request r = {};
+  if (b >= p.requests) return r;
+  r.first = start_of(p, b);
+  const int next = start_of(p, b + 1), length = p.lengths[b];
+  r.rows = max(next - r.first, 0), r.length = max(length, 0);
+  r.tokens = min(r.length, p.places);
+  r.begin = p.window ? max(r.length - r.rows + 1 - p.window, 0) & ~15 : 0;
+  r.blocks = (max(r.tokens - r.begin, 0) + BLOCK - 1) / BLOCK;
+  r.tiles = (r.rows * p.group + (1 << p.plan.tile_log) - 1) >> p.plan.tile_log;
   return r;
 }
 
-// W: dim / 32.  RT: tiles of 16 rows per wavefront.  BY_ROWS: wavefronts have rows of their own; else all have the same rows, and blocks in turn.
-template <bool BF16, int W, int RT, bool BY_ROWS>
-__global__ __launch_bounds__(256) void kv4_attend_kernel(AttendParams p) {
-  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_BYTES = V_BYTES + 2 * 4 * BLOCK, TILE = BY_ROWS ? WAVES * RT * 16 : RT * 16;
-  constexpr int MEET_BYTES = BY_ROWS ? 0 : (WAVES / 2) * RT * 16 * (D + 2) * 4;
-  __shared__ __attribute__((aligned(16))) char lds[MEET_BYTES > WAVES * WAVE_BYTES ? MEET_BYTES : WAVES * WAVE_BYTES];
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), m = lane % 16, g = lane / 16;
-  const int kv_heads = p.cache.heads, item = blockIdx.x / kv_heads, kv = blockIdx.x % kv_heads, slice = blockIdx.y;
+// the sum of v over the lanes up to this one
+__device__ __forceinline__ int sum_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: a row's last to the next one
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: the first half's to the second
+  return v;
+}
 
-  if (p.clear && kv == 0 && slice == 0) {  // rows of no request
-    const int64_t from = p.requests ? start_of(p, 0) : 0, to = p.requests ? start_of(p, p.requests) : 0, others = from + p.tokens - max(from, to), size = (int64_t)p.heads * D;
-    for (int64_t i = item; i < others; i += p.plan.items) {
-      uint16_t *row = (uint16_t *)p.out + (i < from ? i : max(from, to) + i - from) * p.o_token;
+// the work of workgroup `index`; or of the request that holds row `row` of the step, with `index` < 0
+__device__ __forceinline__ Work work_of(const AttendParams &p, int index, int row) {
+  const int lane = threadIdx.x % 64, tile_log = p.plan.tile_log;
+  Request r = request_of(p, lane);
+  int size = 1 << 24;  // of a slice, in blocks: all
+  if (p.plan.extra) {
+    float all = (float)r.tiles * (float)r.blocks;
+    int most = r.blocks;
+    for (int at = 64; at < p.requests; at += 64) {
+      const Request o = request_of(p, at + lane);
+      all += (float)o.tiles * (float)o.blocks, most = max(most, o.blocks);
+    }
+    all = over_lanes<16>(all, [](float a, float b) { return a + b; }), all = over_row(all, [](float a, float b) { return a + b; });
+    const float longest = over_lanes<16>((float)most, [](float a, float b) { return fmaxf(a, b); });
+    // (rounded up past what 32 bits lose: no more slices than there are workgroups)
+    const float each = fmaxf(all * p.plan.over_extra * 1.0001f, over_row(longest, [](float a, float b) { return fmaxf(a, b); }) * (1.0001f / MOST_SLICES));
+    size = ((int)fminf(each, 16777000.f) + 1 + p.plan.round - 1) & ~(p.plan.round - 1);
+  }
+  Work w = {};
+  int before = 0;
+  for (int at = 0; at < p.requests; at += 64) {
+    if (at) r = request_of(p, at + lane);
+    const int slices = r.blocks > size ? (int)((u32)(r.blocks + size - 1) / (u32)size) : 1, count = r.tiles * slices, upto = sum_upto(count);
+    const bool here = index < 0 ? row >= r.first && row < r.first + r.rows : index >= before + upto - count && index < before + upto;
+    const unsigned long long found = __ballot(here);
+    if (found) {
+      const int at_lane = __builtin_ctzll(found);
+      auto get = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at_lane); };
+      w.request = at + at_lane, w.first = get(r.first), w.rows = get(r.rows), w.length = get(r.length), w.tokens = get(r.tokens), w.begin = get(r.begin);
+      w.slices = get(slices), w.index = before + get(upto - count);
+      w.size = size * BLOCK;
+      if (w.slices > 1) {  // slices of one length within the request
+        const u32 blocks = (u32)get(r.blocks);
+        w.size = (int)(((blocks + w.slices - 1) / (u32)w.slices + p.plan.round - 1) & ~(p.plan.round - 1)) * BLOCK;
+      }
+      const int of = index - w.index;
+      w.tile = index < 0 ? ((row - w.first) * p.group) >> tile_log : w.slices > 1 ? (int)((u32)of / (u32)w.slices) : of;
+      w.slice = index < 0 ? 0 : of - w.tile * w.slices;
+      // (only where starts are not in order may it not have that tile, or workgroup)
+      if (w.tile < 0 || w.tile >= get(r.tiles) || w.slice < 0 || w.index < 0 || (int64_t)w.index + (int64_t)(w.tile + 1) * w.slices > p.plan.items + p.plan.extra) w.rows = 0;
+      return w;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return w;
+}
+
+constexpr int most_row_tiles(int w) { return w <= 4 ? 2 : 1; }
+
+// W: dim / 32.  RT: tiles of rows per wavefront, ROWS: of such a tile.  BY_ROWS: wavefronts have rows of their own; else all have the same rows, and blocks in turn.
+// The matrix instructions' tiles have 16 rows.  Of fewer (a token's heads of one key's) each is there 16 / ROWS times, and of the scores that a lane gets so, those of 4
+// tiles of tokens, it goes on with 4 ROWS / 16 of them: the copies share the softmax.
+template <bool BF16, int W, int RT, int ROWS, bool BY_ROWS>
+__global__ __launch_bounds__(256, W > 4 ? 1 : ROWS < 16 ? 3 : 2) void kv4_attend_kernel(AttendParams p) {
+  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK, WAVE_ROWS = RT * ROWS, TILE = (BY_ROWS ? WAVES : 1) * WAVE_ROWS;
+  constexpr int BANKS = 16 / ROWS, NJ = 4 / BANKS;
+  constexpr int MEET_PITCH = D + 4, MEET_BYTES = BY_ROWS ? 0 : WAVES * WAVE_ROWS * (MEET_PITCH + 2) * 4;
+  __shared__ __attribute__((aligned(16))) char lds[MEET_BYTES > WAVES * WAVE_BYTES ? MEET_BYTES : WAVES * WAVE_BYTES];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), m = lane % 16, g = lane / 16, bank = m / ROWS;
+  const int kv_heads = p.cache.heads, groups = (int)(p.plan.items + p.plan.extra) * kv_heads;
+
+  if ((int)blockIdx.x >= groups) {  // rows of no request
+    const int64_t from = p.requests ? start_of(p, 0) : 0, to = max(from, p.requests ? (int64_t)start_of(p, p.requests) : 0), others = from + p.tokens - to, size = (int64_t)p.heads * D;
+    for (int64_t i = blockIdx.x - groups; i < others; i += gridDim.x - groups) {
+      uint16_t *row = (uint16_t *)p.out + (i < from ? i : to + i - from) * p.o_token;
       for (int64_t e = threadIdx.x; e < size; e += 256) row[e / D * p.o_head + e % D] = 0;
     }
+    return;
   }
-  if (!p.requests) return;
-
-  // Tiles of request b are numbered from floor(starts[b] * group / TILE) + b: that leaves room for all of them, whatever the requests before have
-  int b = -1;
-  for (int at = 0; at < p.requests; at += 64) {
-    const bool before = at + lane < p.requests && (int)((int64_t)start_of(p, min(at + lane, p.requests - 1)) * p.group / TILE) + at + lane <= item;
-    b += __popcll(__ballot(before));
-  }
-  b = max(b, 0);
-  const int tile = item - (int)((int64_t)start_of(p, b) * p.group / TILE) - b;
-  const Rows r = rows_of(p, b, tile);
-  if (tile < 0 || (int64_t)tile * TILE >= (int64_t)r.rows * p.group || slice >= r.slices) return;
+  // (the last first: of a prompt's tiles those have the most tokens)
+  const int item = (int)(p.plan.items + p.plan.extra) - 1 - divided(blockIdx.x, p.by_kv_heads), kv = blockIdx.x - (int)(p.plan.items + p.plan.extra - 1 - item) * kv_heads;
+  const Work r = work_of(p, item, 0);
+  if (!r.rows) return;
 
   char *const mine = lds + wave * WAVE_BYTES;
-  u32 *const key_pairs = (u32 *)(mine + V_BYTES), *const value_pairs = key_pairs + BLOCK;
-  const int row0 = tile * TILE + (BY_ROWS ? wave * RT * 16 : 0);  // of the request's tokens and the group's heads
+  float *const key_step = (float *)(mine + V_BYTES), *const key_low = key_step + BLOCK, *const value_step = key_low + BLOCK, *const value_low = value_step + BLOCK;
+  const int row0 = r.tile * TILE + (BY_ROWS ? wave * WAVE_ROWS : 0);  // of the request's tokens and the group's heads
 
-  // The rows: what they see, and q as operands
+  // The rows, what they see, and q, on its way
   int low[RT], high[RT];  // [low, high)
-  int64_t row_at[RT];     // token * heads + head, -1: no row
-  float factor[RT], sum_q[RT];
-  uint4 q[RT][W];
+  bool live[RT];
+  Dwords<4> raw[RT][W];
   for (int t = 0; t < RT; t++) {
-    const int row = row0 + t * 16 + m, token = row / p.group, head = kv * p.group + row % p.group;
-    const bool live = token < r.rows;
-    row_at[t] = live ? (int64_t)(r.first + token) * p.heads + head : -1;
+    const int row = row0 + t * ROWS + m % ROWS, token = divided(row, p.by_group), head = kv * p.group + row - token * p.group;
+    live[t] = token < r.rows;
     const int position = r.length - r.rows + token;
     low[t] = p.window ? max(position - p.window + 1, 0) : 0;
-    high[t] = live ? min(position + 1, r.tokens) : 0;
-    float v[W][8], most = 0.f, sum = 0.f;
-    const char *from = (const char *)p.q + 2 * ((int64_t)(r.first + (live ? token : 0)) * p.q_token + (int64_t)head * p.q_head) + 16 * g * W;
-    for (int w = 0; w < W; w++) {
-      const Dwords<4> x = load_dwords<4>(from + 16 * w);
-      for (int e = 0; e < 8; e++) {
-        v[w][e] = live ? half_of(x.d[e / 2], BF16, e & 1) : 0.f;
-        most = fmaxf(most, fabsf(v[w][e])), sum += v[w][e];
-      }
-    }
-    most = over_row(most, [](float a, float b) { return fmaxf(a, b); });
-    sum = over_row(sum, [](float a, float b) { return a + b; });
-    const float scaled = row_ops::fp16_scale(most);
-    for (int w = 0; w < W; w++) {
-      float x[8];
-      for (int e = 0; e < 8; e++) x[e] = v[w][e] * (e & 2 ? scaled * 0x1p-4f : scaled);
-      q[t][w] = make_uint4(fp16_pair(x[0], x[1]), fp16_pair(x[2], x[3]), fp16_pair(x[4], x[5]), fp16_pair(x[6], x[7]));
-    }
-    factor[t] = p.scale * LOG2_E * 0x1p24f / scaled;
-    // (a row with an infinity: NaN, as the formula gives, also where all its scores are -inf here)
-    sum_q[t] = (sum - sum == 0.f ? sum : __builtin_nanf("")) * p.scale * LOG2_E;
+    high[t] = live[t] ? min(position + 1, r.tokens) : 0;
+    const char *from = (const char *)p.q + 2 * ((int64_t)(r.first + (live[t] ? token : 0)) * p.q_token + (int64_t)head * p.q_head) + 16 * g * W;
+    for (int w = 0; w < W; w++) raw[t][w] = load_dwords<4>(from + 16 * w);
   }
 
   // all of a block's tokens are seen by all of the wavefront's rows where it lies inside [seen_from, seen_to)
-  int seen_from, seen_to, last;
+  int seen_from, seen_to, last, window_begin;  // (the last two: where what any of them sees ends, and begins, at a multiple of 16)
   {
-    const int top = row0 / p.group, bottom = min((row0 + RT * 16 - 1) / p.group, r.rows - 1), behind = r.length - r.rows + 1;
+    const int top = divided(row0, p.by_group), bottom = min(divided(row0 + WAVE_ROWS - 1, p.by_group), r.rows - 1), behind = r.length - r.rows + 1;
     seen_from = p.window ? max(behind + bottom - p.window, 0) : 0;
     seen_to = min(behind + top, r.tokens);
     last = top < r.rows ? min(behind + bottom, r.tokens) : 0;
+    window_begin = p.window ? max(behind + top - p.window, 0) & ~15 : 0;
   }
-  const int begin = r.begin + slice * p.plan.slice, end = min(slice == r.slices - 1 ? r.end : begin + p.plan.slice, last);
+  const int slice_begin = r.begin + r.slice * r.size, end = __builtin_amdgcn_readfirstlane(min(slice_begin + r.size, last)), begin = max(slice_begin, window_begin);
+  seen_from = __builtin_amdgcn_readfirstlane(seen_from), seen_to = __builtin_amdgcn_readfirstlane(min(seen_to, end));
   constexpr int STEP = BY_ROWS ? BLOCK : WAVES * BLOCK;
-  const int start = begin + (BY_ROWS ? 0 : wave * BLOCK);
-  const int blocks = end > start ? (end - start + STEP - 1) / STEP : 0;
+  const int start = __builtin_amdgcn_readfirstlane(begin + (BY_ROWS ? 0 : wave * BLOCK));
+  const int blocks = __builtin_amdgcn_readfirstlane(end > start ? (end - start + STEP - 1) / STEP : 0);
 
   const char *const cache = (const char *)p.cache.base + (int64_t)kv * p.cache.head_bytes;
   const int page = p.cache.page;
+  // the table's entries of 16 blocks: lane 4 n + j has that of tile j of block n
+  int entry = 0, within = 0;
+  unsigned long long there = 0;
+  auto look_up = [&](int n) __attribute__((always_inline)) {
+    const int token = start + (n + lane / 4) * STEP + lane % 4 * 16, column = divided(token, p.cache.by_page);
+    entry = -1;
+    if (token < end) entry = p.table[(int64_t)r.request * p.ld_table + column];  // (end is inside the table)
+    const bool ok = entry >= 0 && entry < p.cache.pages;
+    there = __ballot(ok);
+    entry = ok ? entry : 0, within = token - column * page;
+  };
+  // A block's keys, values and pairs.  Those of the next one are asked for as soon as the registers of this one's are free: values and pairs once they are in
+  // LDS, keys behind their products.
+  Dwords<W> keys[4], values[4];
+  u32 key_pair, value_pair;
+  int64_t tiles[4];  // where they begin
+  auto find = [&](int n) __attribute__((always_inline)) {
+    if (n % 16 == 0) look_up(n);
+    for (int j = 0; j < 4; j++) {
+      const int at = n % 16 * 4 + j;
+      tiles[j] = (int64_t)__builtin_amdgcn_readlane(entry, at) * p.cache.page_bytes + (int64_t)__builtin_amdgcn_readlane(within, at) * (D / 2);
+    }
+  };
+  const char *const codes = cache + m * (D / 2) + g * (4 * W);
+  auto load_keys = [&]() __attribute__((always_inline)) {
+    for (int j = 0; j < 4; j++) keys[j] = load_dwords<W>(codes + tiles[j]);
+  };
+  auto load_values = [&](int n) __attribute__((always_inline)) {
+    for (int j = 0; j < 4; j++) values[j] = load_dwords<W>(codes + (int64_t)page * (D / 2) + tiles[j]);
+    const int at = n % 16 * 4 + g, token = start + n * STEP + lane;
+    const char *pairs = cache + (int64_t)__shfl(entry, at) * p.cache.page_bytes + (int64_t)page * D + (__shfl(within, at) + m) * 4;
+    key_pair = *(const u32 *)pairs, value_pair = *(const u32 *)(pairs + page * 4);
+    if (token >= end || !(there >> at & 1)) key_pair = value_pair = 0;  // (memory that was never written may hold any)
+  };
+
+  if (blocks) {
+    find(0);
+    load_values(0);
+    load_keys();
+  }
+  // q as operands
+  float factor[RT], sum_q[RT];  // scores (in powers of two) are factor * (codes' product * step + lowest * sum_q)
+  uint4 q[RT][W];
+  for (int t = 0; t < RT; t++) {
+    float v[W][8], most = 0.f, sum = 0.f;
+    for (int w = 0; w < W; w++)
+      for (int e = 0; e < 8; e++) {
+        v[w][e] = live[t] ? half_of(raw[t][w].d[e / 2], BF16, e & 1) : 0.f;
+        most = fmaxf(most, fabsf(v[w][e])), sum += v[w][e];
+      }
+    most = over_row(most, [](float a, float b) { return fmaxf(a, b); });
+    sum = over_row(sum, [](float a, float b) { return a + b; });
+    const float scaled = row_ops::fp16_scale(most), sign = p.scale < 0.f ? -scaled : p.scale == 0.f ? 0.f : scaled;
+    for (int w = 0; w < W; w++) {
+      float x[8];
+      for (int e = 0; e < 8; e++) x[e] = v[w][e] * (e & 2 ? sign * 0x1p-4f : sign);
+      q[t][w] = make_uint4(fp16_pair(x[0], x[1]), fp16_pair(x[2], x[3]), fp16_pair(x[4], x[5]), fp16_pair(x[6], x[7]));
+    }
+    factor[t] = fmaxf(fabsf(p.scale) * LOG2_E * 0x1p24f / scaled, 0x1p-126f);
+    // (a row with an infinity: NaN, as the formula gives, also where all its scores are -inf here)
+    sum_q[t] = (sum - sum == 0.f ? sum : __builtin_nanf("")) * sign * 0x1p-24f;
+  }
   f32x4 out[D / 16][RT];
   float top[RT], total[RT], lowest[RT];
   for (int t = 0; t < RT; t++) {
     top[t] = -__builtin_inff(), total[t] = 0.f, lowest[t] = 0.f;
     for (int d = 0; d < D / 16; d++) out[d][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  int power = -112;  // values' steps are below 2^power
-
-  // the table's entries of 16 blocks: lane 4 n + j has that of tile j of block n
-  int entry = 0, within = 0;
-  unsigned long long there = 0;
-  auto look_up = [&](int n) __attribute__((always_inline)) {
-    const int token = start + (n + lane / 4) * STEP + lane % 4 * 16, column = token / page;
-    entry = -1;
-    if (token < end) entry = p.table[(int64_t)r.request * p.ld_table + column];  // (end is inside the table)
-    const bool ok = entry >= 0 && entry < p.cache.pages;
-    there = __ballot(ok);
-    entry = ok ? entry : 0, within = token % page;
-  };
-  struct Block {
-    Dwords<W> k[4], v[4];
-    u32 kp, vp;
-  };
-  auto load_block = [&](int n) __attribute__((always_inline)) {
-    Block x;
-    for (int j = 0; j < 4; j++) {
-      const int at = n % 16 * 4 + j;
-      const int64_t of = (int64_t)__builtin_amdgcn_readlane(entry, at) * p.cache.page_bytes + (int64_t)__builtin_amdgcn_readlane(within, at) * (D / 2);
-      const char *codes = cache + of + m * (D / 2) + g * (4 * W);
-      x.k[j] = load_dwords<W>(codes), x.v[j] = load_dwords<W>(codes + (int64_t)page * (D / 2));
-    }
-    const int at = n % 16 * 4 + g, token = start + n * STEP + lane;
-    const char *pairs = cache + (int64_t)__shfl(entry, at) * p.cache.page_bytes + (int64_t)page * D + (__shfl(within, at) + m) * 4;
-    x.kp = *(const u32 *)pairs, x.vp = *(const u32 *)(pairs + page * 4);
-    if (token >= end || !(there >> at & 1)) x.kp = x.vp = 0;  // (memory that was never written may hold any)
-    return x;
-  };
+  int power = -112;  // values' steps so far are up to 2^power
+  float unit = __builtin_amdgcn_ldexpf(1.f, 14 - power), limit = __builtin_amdgcn_ldexpf(1.f, power);
 
   for (int n = 0; n < blocks; n++) {
-    if (n % 16 == 0) look_up(n);
-    const Block x = load_block(n);
+    const u32 present = (u32)(there >> (n % 16 * 4)) & 15;  // tiles
     // values and pairs to LDS: the 16 tokens of a lane's operand in a row, 8 bytes between rows
-    for (int j = 0; j < 4; j++) __builtin_memcpy(mine + (m / 4 * 16 + j * 4 + m % 4) * PITCH + g * (4 * W), &x.v[j], 4 * W);
-    key_pairs[lane] = x.kp, value_pairs[lane] = x.vp;
+    for (int j = 0; j < 4; j++) __builtin_memcpy(mine + (m / 4 * 16 + j * 4 + m % 4) * PITCH + g * (4 * W), &values[j], 4 * W);
+    const float step = half_of(value_pair, BF16, false), lowest_value = half_of(value_pair, BF16, true);
+    if (__any(step > limit && step < __builtin_inff())) {  // the largest so far: what there is in its unit
+      const float most = over_lanes<64>(step < __builtin_inff() ? step : 0.f, [](float a, float b) { return fmaxf(a, b); });
+      const int now = __builtin_amdgcn_frexp_expf(most);
+      const float moved = __builtin_amdgcn_ldexpf(1.f, max(power - now, -126));
+      for (int t = 0; t < RT; t++)
+        for (int d = 0; d < D / 16; d++)
+          for (int i = 0; i < 4; i++) out[d][t][i] *= moved;
+      power = now, unit = __builtin_amdgcn_ldexpf(1.f, 14 - power), limit = __builtin_amdgcn_ldexpf(1.f, power);
+    }
+    key_step[lane] = half_of(key_pair, BF16, false), key_low[lane] = half_of(key_pair, BF16, true);
+    value_step[lane] = step * (lane & 1 ? unit * 0x1p-4f : unit), value_low[lane] = lowest_value;
+    const int first = start + n * STEP;
+    const bool whole = first >= seen_from && first + BLOCK <= seen_to && present == 15;
+    // a step or lowest value of NaN stays with the rows that see it: 0 times it is not 0
+    const bool careful = !whole && __any(!(fabsf(step) + fabsf(lowest_value) < __builtin_inff()));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    f32x4 s[4][RT];
-    for (int j = 0; j < 4; j++) {
-      for (int t = 0; t < RT; t++) s[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int w = 0; w < W; w++) {
-        const uint4 k = codes_of(x.k[j].d[w]);
-        for (int t = 0; t < RT; t++) s[j][t] = mfma16<false>(k, q[t][w], s[j][t]);
-      }
+    if (n + 1 < blocks) {
+      find(n + 1);
+      load_values(n + 1);
     }
-    float value_step[4][4], value_low[4][4], most_step = 0.f;
-    for (int j = 0; j < 4; j++) {
-      const uint4 kp = *(const uint4 *)(key_pairs + 16 * j + 4 * g), vp = *(const uint4 *)(value_pairs + 16 * j + 4 * g);
-      const u32 k[4] = {kp.x, kp.y, kp.z, kp.w}, v[4] = {vp.x, vp.y, vp.z, vp.w};
-      for (int i = 0; i < 4; i++) {
-        const float step = half_of(k[i], BF16, false), low_k = half_of(k[i], BF16, true);
-        for (int t = 0; t < RT; t++) s[j][t][i] = s[j][t][i] * factor[t] * step + low_k * sum_q[t];
-        value_step[j][i] = half_of(v[i], BF16, false), value_low[j][i] = half_of(v[i], BF16, true);
-        most_step = fmaxf(most_step, value_step[j][i]);
+
+    f32x4 s[NJ][RT];  // of tiles NJ * bank ..
+    {
+      f32x4 all[4][RT];
+      for (int j = 0; j < 4; j++) {
+        for (int t = 0; t < RT; t++) all[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < W; w++) {
+          const uint4 k = codes_of(keys[j].d[w]);
+          for (int t = 0; t < RT; t++) all[j][t] = mfma16<false>(k, q[t][w], all[j][t]);
+        }
       }
+      for (int t = 0; t < RT; t++)
+        for (int j = 0; j < NJ; j++)
+          for (int i = 0; i < 4; i++) {
+            s[j][t][i] = all[j][t][i];
+            for (int b = 1; b < BANKS; b++) s[j][t][i] = bank == b ? all[NJ * b + j][t][i] : s[j][t][i];
+          }
     }
-    const int first = start + n * STEP;
-    const bool whole = first >= seen_from && first + BLOCK <= seen_to && (there >> (n % 16 * 4) & 15) == 15;
-    u32 seen[RT];
-    for (int t = 0; t < RT; t++) seen[t] = 0xffff;
+    if (n + 1 < blocks) load_keys();
+    const int at = 16 * NJ * bank + 4 * g;  // the first of a lane's tokens in the block
+    for (int j = 0; j < NJ; j++) {
+      const f32x4 step_k = *(const f32x4 *)(key_step + at + 16 * j), low_k = *(const f32x4 *)(key_low + at + 16 * j);
+      for (int t = 0; t < RT; t++)
+        for (int i = 0; i < 4; i++) s[j][t][i] = __builtin_fmaf(s[j][t][i], step_k[i], low_k[i] * sum_q[t]);
+    }
     if (!whole)
       for (int t = 0; t < RT; t++) {
-        seen[t] = 0;
-        for (int j = 0; j < 4; j++)
-          for (int i = 0; i < 4; i++) {
-            const int token = first + 16 * j + 4 * g + i;
-            const bool ok = token >= low[t] && token < min(high[t], end) && (there >> (n % 16 * 4 + j) & 1);
-            seen[t] |= (u32)ok << (4 * j + i);
-            s[j][t][i] = ok ? s[j][t][i] : -__builtin_inff();
-          }
+        const int from = low[t] - first - at, to = min(high[t], end) - first - at;
+        for (int j = 0; j < NJ; j++)
+          for (int i = 0; i < 4; i++) s[j][t][i] = 16 * j + i >= from && 16 * j + i < to && (present >> (NJ * bank + j) & 1) ? s[j][t][i] : -__builtin_inff();
       }
-    most_step = over_row(most_step, [](float a, float b) { return fmaxf(a, b); });
-    const int power_now = most_step > 0.f && most_step < __builtin_inff() ? max(power, __builtin_amdgcn_frexp_expf(most_step)) : power;
-    const float unit = __builtin_amdgcn_ldexpf(1.f, 14 - power_now);
-    for (int j = 0; j < 4; j++)
-      for (int i = 0; i < 4; i++) value_step[j][i] *= unit * (i & 1 ? 0x1p-4f : 1.f);
-    uint4 weights[2][RT];
+    uint4 weights[RT][BF16 ? 1 : 2][2];
     for (int t = 0; t < RT; t++) {
       float most = -__builtin_inff();
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < NJ; j++)
         for (int i = 0; i < 4; i++) most = fmaxf(most, s[j][t][i]);
-      most = fmaxf(top[t], over_row(most, [](float a, float b) { return fmaxf(a, b); }));
-      const float from = most == -__builtin_inff() ? 0.f : most;  // (nothing seen yet)
-      const float kept = __builtin_amdgcn_exp2f(top[t] - from);
-      top[t] = most;
-      total[t] *= kept, lowest[t] *= kept;
-      const float moved = __builtin_amdgcn_ldexpf(kept, power - power_now);
-      for (int d = 0; d < D / 16; d++)
-        for (int i = 0; i < 4; i++) out[d][t][i] *= moved;
-      float weight[4][4];
-      for (int j = 0; j < 4; j++)
-        for (int i = 0; i < 4; i++) {
-          const bool ok = seen[t] >> (4 * j + i) & 1;
-          const float e = __builtin_amdgcn_exp2f(s[j][t][i] - from);
-          total[t] += e;
-          // (a step or lowest value of NaN stays with the rows that see it)
-          lowest[t] += ok ? e * value_low[j][i] : 0.f;
-          weight[j][i] = ok ? e * value_step[j][i] : 0.f;
+      most = fmaxf(top[t], over_row<ROWS>(most, [](float a, float b) { return fmaxf(a, b); }));
+      const float from = most == -__builtin_inff() ? 0.f : most, shift = -from * factor[t];  // (-inf: nothing seen yet)
+      if (__any(most != top[t])) {
+        const float kept = __builtin_amdgcn_exp2f((top[t] - from) * factor[t]);
+        total[t] *= kept, lowest[t] *= kept;
+        for (int d = 0; d < D / 16; d++)
+          for (int i = 0; i < 4; i++) out[d][t][i] *= kept;
+        top[t] = most;
+      }
+      float sum = 0.f, base = 0.f;
+      auto weigh = [&](auto checked) __attribute__((always_inline)) {
+        constexpr int J = NJ < 2 ? 1 : 2;  // tiles of a pair that are the lane's own
+        // pairs of tiles 0 and 1, and of 2 and 3, into the lanes of bank 0 (the others' columns of `out` hold nothing of use)
+        for (int h = 0; h < NJ / J; h++) {
+          float e[2][4], st[2][4];
+          for (int j = 0; j < J; j++) {
+            const f32x4 step_v = *(const f32x4 *)(value_step + at + 16 * (2 * h + j)), low_v = *(const f32x4 *)(value_low + at + 16 * (2 * h + j));
+            for (int i = 0; i < 4; i++) {
+              const float score = s[2 * h + j][t][i];
+              const bool ok = !decltype(checked)::value || score != -__builtin_inff();
+              e[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score, factor[t], shift));
+              st[j][i] = ok ? step_v[i] : 0.f;
+              sum += e[j][i];
+              base = __builtin_fmaf(e[j][i], ok ? low_v[i] : 0.f, base);
+            }
+          }
+          u32 w[4], rest[4];
+          for (int i = 0; i < 4; i++) {
+            const float a = e[0][i] * st[0][i], b = J == 1 ? dpp_moved<0x104>(a) : e[J - 1][i] * st[J - 1][i];  // (row_shl 4)
+            const tts_gemm_device::f16x2 pair = {(_Float16)a, (_Float16)b};
+            w[i] = __builtin_bit_cast(u32, pair);
+            if constexpr (!BF16) {
+              const float ra = __builtin_fmaf(e[0][i], st[0][i], -(float)pair[0]);
+              rest[i] = fp16_pair(ra, J == 1 ? dpp_moved<0x104>(ra) : __builtin_fmaf(e[J - 1][i], st[J - 1][i], -(float)pair[1]));
+            }
+          }
+          weights[t][0][h] = make_uint4(w[0], w[1], w[2], w[3]);
+          if constexpr (!BF16) weights[t][1][h] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
         }
-      for (int h = 0; h < 2; h++)
-        weights[h][t] = make_uint4(fp16_pair(weight[2 * h][0], weight[2 * h + 1][0]), fp16_pair(weight[2 * h][1], weight[2 * h + 1][1]), fp16_pair(weight[2 * h][2], weight[2 * h + 1][2]),
-                                   fp16_pair(weight[2 * h][3], weight[2 * h + 1][3]));
+        if constexpr (NJ < 4)
+          for (int part = 0; part < (BF16 ? 1 : 2); part++) {
+            const uint4 w = weights[t][part][0];
+            weights[t][part][1] = make_uint4(dpp_moved<0x108>(w.x), dpp_moved<0x108>(w.y), dpp_moved<0x108>(w.z), dpp_moved<0x108>(w.w));  // row_shl 8
+          }
+      };
+      if (careful) weigh(std::true_type{});
+      else weigh(std::false_type{});
+      total[t] += sum, lowest[t] += base;
     }
-    power = power_now;
     for (int d = 0; d < D / 16; d++) {
       const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32((i32x2 __attribute__((address_space(3))) *)((__attribute__((address_space(3))) void *)(mine + lane * PITCH + 8 * d)));
-      const uint4 first_half = codes_of(v[0]), second_half = codes_of(v[1]);
-      for (int t = 0; t < RT; t++) out[d][t] = mfma16<false>(first_half, weights[0][t], out[d][t]);
-      for (int t = 0; t < RT; t++) out[d][t] = mfma16<false>(second_half, weights[1][t], out[d][t]);
+      for (int h = 0; h < 2; h++) {
+        const uint4 c = codes_of(v[h]);
+        for (int part = 0; part < (BF16 ? 1 : 2); part++)
+          for (int t = 0; t < RT; t++) out[d][t] = mfma16<false>(c, weights[t][part][h], out[d][t]);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -284,100 +405,123 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendParams p) {
 
   for (int t = 0; t < RT; t++) {
     const auto add = [](float a, float b) { return a + b; };
-    total[t] = over_row(total[t], add), lowest[t] = over_row(lowest[t], add);
+    total[t] = over_row<ROWS>(total[t], add), lowest[t] = over_row<ROWS>(lowest[t], add), top[t] *= factor[t];
     for (int d = 0; d < D / 16; d++)
       for (int i = 0; i < 4; i++) out[d][t][i] = __builtin_amdgcn_ldexpf(out[d][t][i], 10 + power) + lowest[t];
   }
-  if constexpr (!BY_ROWS) {  // the wavefronts' parts, two to two and one to one
-    constexpr int PART = RT * 16 * (D + 2) * 4;
-    for (int half = WAVES / 2; half >= 1; half /= 2) {
-      __syncthreads();
-      if (wave >= half && wave < 2 * half) {
-        float *to = (float *)(lds + (wave - half) * PART);
-        for (int t = 0; t < RT; t++) {
-          for (int d = 0; d < D / 16; d++) *(f32x4 *)(to + (t * (D / 16) + d) * 256 + lane * 4) = out[d][t];
-          if (g == 0) to[RT * 16 * D + t * 16 + m] = top[t], to[RT * 16 * D + RT * 16 + t * 16 + m] = total[t];
-        }
-      }
-      __syncthreads();
-      if (wave < half) {
-        const float *from = (const float *)(lds + wave * PART);
-        for (int t = 0; t < RT; t++) {
-          const float other = from[RT * 16 * D + t * 16 + m], more = from[RT * 16 * D + RT * 16 + t * 16 + m];
-          const float most = fmaxf(top[t], other), base = most == -__builtin_inff() ? 0.f : most;
-          const float here = __builtin_amdgcn_exp2f(top[t] - base), there_too = __builtin_amdgcn_exp2f(other - base);
-          top[t] = most, total[t] = total[t] * here + more * there_too;
-          for (int d = 0; d < D / 16; d++) {
-            const f32x4 add = *(const f32x4 *)(from + (t * (D / 16) + d) * 256 + lane * 4);
-            for (int i = 0; i < 4; i++) out[d][t][i] = out[d][t][i] * here + add[i] * there_too;
-          }
-        }
-      }
-    }
-    if (wave != 0) return;
-  }
-  for (int t = 0; t < RT; t++) {
-    if (row_at[t] < 0) continue;
+  // four elements of a row of the tile
+  const int tile0 = r.tile * TILE, part0 = r.index + r.tile * r.slices + r.slice;
+  auto put = [&](int row, int element, f32x4 v, float most, float sum) __attribute__((always_inline)) {
+    const int token = divided(tile0 + row, p.by_group), head = kv * p.group + tile0 + row - token * p.group;
+    if (token >= r.rows) return;
     if (r.slices == 1) {
-      const float over = total[t] == 0.f ? 0.f : 1.f / total[t];  // (a row that sees nothing: zeros)
-      const int64_t token = row_at[t] / p.heads, head = row_at[t] % p.heads;
-      char *to = (char *)p.out + 2 * (token * p.o_token + head * p.o_head) + 8 * g;
-      for (int d = 0; d < D / 16; d++) {
-        u32 w[2];
-        for (int i = 0; i < 2; i++) {
-          const float a = out[d][t][2 * i] * over, c = out[d][t][2 * i + 1] * over;
-          w[i] = BF16 ? (u32)__builtin_bit_cast(uint16_t, (__bf16)a) | (u32)__builtin_bit_cast(uint16_t, (__bf16)c) << 16 : fp16_pair(a, c);
-        }
-        __builtin_memcpy(to + 32 * d, w, 8);
+      const float over = sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees nothing: zeros)
+      u32 w[2];
+      for (int i = 0; i < 2; i++) {
+        const float a = v[2 * i] * over, c = v[2 * i + 1] * over;
+        w[i] = BF16 ? (u32)__builtin_bit_cast(uint16_t, (__bf16)a) | (u32)__builtin_bit_cast(uint16_t, (__bf16)c) << 16 : fp16_pair(a, c);
       }
+      __builtin_memcpy((char *)p.out + 2 * ((int64_t)(r.first + token) * p.o_token + head * p.o_head + element), w, 8);
     } else {
-      const int64_t part = row_at[t] * p.plan.slices + slice;
-      for (int d = 0; d < D / 16; d++) *(f32x4 *)(p.parts + part * D + 16 * d + 4 * g) = out[d][t];
-      if (g == 0) p.stats[part * 2] = top[t], p.stats[part * 2 + 1] = total[t];
+      const int64_t part = ((int64_t)part0 * kv_heads + kv) * TILE + row;
+      *(f32x4 *)(p.parts + part * D + element) = v;
+      if (element == 0) p.stats[part * 2] = most, p.stats[part * 2 + 1] = sum;
+    }
+  };
+  if constexpr (BY_ROWS) {
+    for (int t = 0; t < RT; t++)
+      for (int d = 0; d < D / 16; d++) put(wave * WAVE_ROWS + t * 16 + m, 16 * d + 4 * g, out[d][t], top[t], total[t]);
+  } else {  // the wavefronts' parts meet in LDS
+    float *const rows = (float *)lds, *const tops = rows + WAVES * WAVE_ROWS * MEET_PITCH, *const totals = tops + WAVES * WAVE_ROWS;
+    __syncthreads();
+    if (bank == 0)
+      for (int t = 0; t < RT; t++) {
+        const int row = wave * WAVE_ROWS + t * ROWS + m;
+        for (int d = 0; d < D / 16; d++) *(f32x4 *)(rows + row * MEET_PITCH + 16 * d + 4 * g) = out[d][t];
+        if (g == 0) tops[row] = top[t], totals[row] = total[t];
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < WAVE_ROWS * (D / 4); i += 256) {
+      const int row = i / (D / 4), element = i % (D / 4) * 4;
+      float most = tops[row], sum = 0.f;
+      for (int w = 1; w < WAVES; w++) most = fmaxf(most, tops[w * WAVE_ROWS + row]);
+      const float base = most == -__builtin_inff() ? 0.f : most;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < WAVES; w++) {
+        const float share = __builtin_amdgcn_exp2f(tops[w * WAVE_ROWS + row] - base);
+        sum += totals[w * WAVE_ROWS + row] * share;
+        const f32x4 part = *(const f32x4 *)(rows + (w * WAVE_ROWS + row) * MEET_PITCH + element);
+        for (int e = 0; e < 4; e++) v[e] += part[e] * share;
+      }
+      put(row, element, v, most, sum);
     }
   }
 }
 
-// The slices of a row, where there are several: a wavefront per row, in the order of the slices.
+// The slices of a row, where there are several, added up in their order: a workgroup per row, four elements a thread and as many slices side by side as that leaves.
 template <bool BF16>
 __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
-  const int lane = threadIdx.x % 64, dim = p.cache.dim;
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64, token = row / p.heads;
-  if (token >= p.tokens) return;
-  const int head = (int)(row % p.heads);
-  int b = -1;
-  for (int at = 0; at < p.requests; at += 64) b += __popcll(__ballot(at + lane < p.requests && start_of(p, min(at + lane, p.requests - 1)) <= token));
-  if (b < 0) return;
-  const int first = start_of(p, b);
-  if (token >= start_of(p, b + 1)) return;  // (a row of no request)
-  const Rows r = rows_of(p, b, (int)(((token - first) * p.group + head % p.group) / p.plan.tile));
-  if (r.slices == 1) return;  // (written already)
-  const float *stats = p.stats + row * p.plan.slices * 2, *parts = p.parts + row * p.plan.slices * dim;
-  float most = -__builtin_inff();
-  for (int i = 0; i < r.slices; i++) most = fmaxf(most, stats[2 * i]);
-  const float base = most == -__builtin_inff() ? 0.f : most;
-  float total = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < r.slices; i++) {
-    const float share = __builtin_amdgcn_exp2f(stats[2 * i] - base);
-    total += stats[2 * i + 1] * share;
-    for (int n = 0; n < 4; n++)
-      if (lane + 64 * n < dim) sum[n] += parts[(int64_t)i * dim + lane + 64 * n] * share;
+  __shared__ float shares[MOST_SLICES];
+  __shared__ f32x4 sums[256];
+  const int tid = threadIdx.x, lane = tid % 64, dim = p.cache.dim;
+  const int token = divided(blockIdx.x, p.by_heads), head = blockIdx.x - token * p.heads;
+  const Work r = work_of(p, -1, token);
+  if (!r.rows || r.slices == 1) return;  // a row of no request, or written already
+  const int kv = divided(head, p.by_group), in_request = (token - r.first) * p.group + head - kv * p.group, tile = 1 << p.plan.tile_log;
+  const int64_t part_step = (int64_t)p.cache.heads * tile;  // from slice to slice
+  const int64_t index = r.index + (int64_t)(in_request >> p.plan.tile_log) * r.slices;
+  if (index + r.slices > p.plan.items + p.plan.extra) return;  // (only where starts are not in order)
+  const int64_t first = (index * p.cache.heads + kv) * tile + (in_request & (tile - 1));
+  const float *stats = p.stats + first * 2, *parts = p.parts + first * dim;
+  const int four = dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64, at = tid % four, side = 256 / four;  // threads per slice, their element, slices at a time
+  f32x4 part = {0.f, 0.f, 0.f, 0.f};
+  if (tid / four < r.slices && 4 * at < dim) part = *(const f32x4 *)(parts + (tid / four) * part_step * dim + 4 * at);
+  // (every wavefront for itself)
+  float top[2], total[2], most = -__builtin_inff(), all = 0.f;
+  for (int h = 0; h < 2; h++) {
+    const int i = lane + 64 * h;
+    top[h] = i < r.slices ? stats[2 * i * part_step] : -__builtin_inff(), total[h] = i < r.slices ? stats[2 * i * part_step + 1] : 0.f;
+    most = fmaxf(most, top[h]);
   }
-  const float over = total == 0.f ? 0.f : 1.f / total;
-  uint16_t *to = (uint16_t *)p.out + token * p.o_token + head * p.o_head;
-  for (int n = 0; n < 4; n++)
-    if (lane + 64 * n < dim) to[lane + 64 * n] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)(sum[n] * over)) : __builtin_bit_cast(uint16_t, (_Float16)(sum[n] * over));
+  most = over_lanes<64>(most, [](float a, float b) { return fmaxf(a, b); });
+  const float base = most == -__builtin_inff() ? 0.f : most;
+  for (int h = 0; h < 2; h++) {
+    const float share = __builtin_amdgcn_exp2f(top[h] - base);
+    all += total[h] * share;
+    if (tid < 64) shares[lane + 64 * h] = share;
+  }
+  all = over_lanes<64>(all, [](float a, float b) { return a + b; });
+  __syncthreads();
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = tid / four; i < r.slices; i += side) {
+    f32x4 next = part;
+    if (i + side < r.slices && 4 * at < dim) next = *(const f32x4 *)(parts + (i + side) * part_step * dim + 4 * at);
+    for (int e = 0; e < 4; e++) sum[e] += part[e] * shares[i];
+    part = next;
+  }
+  sums[tid] = sum;
+  __syncthreads();
+  if (tid >= four || 4 * at >= dim) return;
+  for (int i = 1; i < min(side, r.slices); i++)
+    for (int e = 0; e < 4; e++) sum[e] += sums[tid + i * four][e];
+  const float over = all == 0.f ? 0.f : 1.f / all;
+  uint16_t out[4];
+  for (int e = 0; e < 4; e++) out[e] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)(sum[e] * over)) : __builtin_bit_cast(uint16_t, (_Float16)(sum[e] * over));
+  __builtin_memcpy((uint16_t *)p.out + (int64_t)token * p.o_token + head * p.o_head + 4 * at, out, sizeof out);
 }
 
 template <bool BF16, int W>
 hipError_t launch_of(const AttendParams &p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.plan.items * p.cache.heads), (unsigned)p.plan.slices);
-  if (p.plan.by_rows) kv4_attend_kernel<BF16, W, 2, true><<<grid, 256, 0, s>>>(p);
-  else if (p.plan.row_tiles == 2) kv4_attend_kernel<BF16, W, 2, false><<<grid, 256, 0, s>>>(p);
-  else kv4_attend_kernel<BF16, W, 1, false><<<grid, 256, 0, s>>>(p);
+  const dim3 grid((unsigned)((p.plan.items + p.plan.extra) * p.cache.heads + (p.clear ? 8 : 0)));
+  constexpr int MOST = most_row_tiles(W);
+  if (p.plan.by_rows) kv4_attend_kernel<BF16, W, MOST, 16, true><<<grid, 256, 0, s>>>(p);
+  else if (p.plan.tile_log == 2) kv4_attend_kernel<BF16, W, 1, 4, false><<<grid, 256, 0, s>>>(p);
+  else if (p.plan.tile_log == 3) kv4_attend_kernel<BF16, W, 1, 8, false><<<grid, 256, 0, s>>>(p);
+  else if (p.plan.tile_log == 4) kv4_attend_kernel<BF16, W, 1, 16, false><<<grid, 256, 0, s>>>(p);
+  else kv4_attend_kernel<BF16, W, MOST, 16, false><<<grid, 256, 0, s>>>(p);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.plan.slices > 1) {
-    kv4_attend_join_kernel<BF16><<<dim3((unsigned)((p.tokens * p.heads + 3) / 4)), 256, 0, s>>>(p);
+  if (e == hipSuccess && p.plan.extra) {
+    kv4_attend_join_kernel<BF16><<<dim3((unsigned)(p.tokens * p.heads)), 256, 0, s>>>(p);
     e = hipGetLastError();
   }
   return e;
@@ -403,20 +547,24 @@ AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, in
   AttendPlan plan = {};
   const int64_t group = heads / kv_heads, rows = (tokens + requests - 1) / std::max(requests, 1) * group;  // of a request, on average
   plan.by_rows = rows > 64;
-  plan.row_tiles = rows > 16 ? 2 : 1;
-  plan.tile = plan.by_rows ? WAVES * plan.row_tiles * 16 : plan.row_tiles * 16;
-  plan.items = std::max<int64_t>(1, tokens * group / plan.tile + requests);
-  const int64_t range = window ? std::min<int64_t>(longest, (int64_t)window + plan.tile / group + 17) : longest;
-  const int64_t groups = std::max<int64_t>(1, plan.items * kv_heads), wanted = 1024;
-  const int64_t least = WAVES * BLOCK;  // tokens of a slice
-  int64_t slices = std::max<int64_t>(1, std::min((wanted + groups - 1) / groups, (range + least - 1) / least));
-  plan.slice = (int)std::max<int64_t>(((range + slices - 1) / slices + least - 1) / least * least, least);
-  plan.slices = (int)std::max<int64_t>(1, (range + plan.slice - 1) / plan.slice);
+  const int most = most_row_tiles(dim / 32) * 16;
+  const int tile = plan.by_rows ? WAVES * most : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : most;
+  plan.tile_log = __builtin_ctz(tile);
+  // tiles: each request's rows rounded up, which is what they are where a token's rows fill whole tiles
+  plan.items = std::max<int64_t>(1, group % tile == 0 ? tokens * (group / tile) : (tokens * group + (int64_t)requests * (tile - 1)) / tile);
+  const int64_t range = window ? std::min<int64_t>(longest, (int64_t)window + tile / group + 17) : longest;
+  const int64_t wanted = plan.by_rows ? 256 : 512;
+  plan.round = plan.by_rows ? 1 : WAVES;
+  if (range > (plan.by_rows ? 4 : 1) * WAVES * BLOCK && (!plan.by_rows || plan.items * kv_heads < 256)) {
+    const int64_t most_extra = plan.items * std::min<int64_t>((range + BLOCK - 1) / BLOCK / plan.round, MOST_SLICES);  // (more than that has nothing to do)
+    plan.extra = std::max<int64_t>(0, std::min((wanted + kv_heads - 1) / kv_heads, most_extra));
+    plan.over_extra = plan.extra ? 1.f / (float)plan.extra : 0.f;
+  }
   return plan;
 }
 
-size_t attend_workspace_bytes(const AttendPlan &plan, int64_t tokens, int heads, int dim) {
-  return plan.slices > 1 ? (size_t)tokens * heads * plan.slices * (dim + 2) * sizeof(float) : 0;
+size_t attend_workspace_bytes(const AttendPlan &plan, int kv_heads, int dim) {
+  return plan.extra ? (size_t)(plan.items + plan.extra) * (kv_heads * (dim + 2) * sizeof(float) << plan.tile_log) : 0;
 }
 
 hipError_t launch_attend(const AttendParams &p, hipStream_t s) { return p.cache.bf16 ? launch_as<true>(p, s) : launch_as<false>(p, s); }

@@ -30,10 +30,10 @@ __device__ __forceinline__ Packed<T, V> load(const T *p) {
 template <class T, int V, bool INTER, int L, int N, int H>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeParams p) {
   const int heads = p.heads + p.kv_heads, chunks = (heads + H - 1) / H, units = p.dim / (2 * V), turned = p.rotary / (2 * V);
-  const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, items = p.tokens * chunks;
-  const int lane = threadIdx.x % L;
-  const int64_t t = min(item / chunks, p.tokens - 1);
-  const int chunk = (int)(item % chunks), position = p.positions[t];
+  const int item = blockIdx.x * (256 / L) + threadIdx.x / L, items = (int)p.tokens * chunks, lane = threadIdx.x % L;
+  const int token = divided(item, p.by_chunks), chunk = item - token * chunks;
+  const int64_t t = min(token, (int)p.tokens - 1);
+  const int position = p.positions[t];
   const bool there = position >= 0 && position < p.places;
   if (item >= items || (!there && !p.clear)) return;  // (all lanes of a head)
   const float *turn = p.cos_sin + (there ? position : 0) * p.ld_cos_sin;
@@ -100,6 +100,7 @@ hipError_t go(const RopeParams &p, hipStream_t s) {
   const int64_t each = most * per / chunks;                                                          // tokens (a launch has less than 2^32 lanes)
   for (int64_t at = 0; at < p.tokens; at += each) {
     RopeParams part = p;
+    part.by_chunks = fast_div((uint32_t)chunks);
     part.tokens = std::min(each, p.tokens - at);
     part.positions += at;
     part.q = (const T *)p.q + at * p.q_token, part.k = (const T *)p.k + at * p.k_token;
