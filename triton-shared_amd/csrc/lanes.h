@@ -8,7 +8,7 @@ template <int CTRL, class T>
 __device__ __forceinline__ T dpp_moved(T v) {
   static_assert(sizeof(T) == 4, "");
   const int d = __builtin_bit_cast(int, v);
-  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(d, d, CTRL, 0xf, 0xf, false));
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, d, CTRL, 0xf, 0xf, true));  // (0 where there is no such lane)
 }
 
 // f over groups of G neighbouring lanes, in all of them: up to 16 lanes by DPP moves, which read lanes of the group alone

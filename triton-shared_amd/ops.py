@@ -216,7 +216,7 @@ def page_slots(table, lengths, fresh, free, count, page, rows):
     if rows < 0:
         raise ValueError(f"rows is {rows}")
     sizes = (rows, rows, rows, table.shape[0] + 1, 1)
-    made = tuple(torch.empty(n, dtype=torch.int32, device=device) for n in sizes)
+    made = torch.empty(sum(sizes), dtype=torch.int32, device=device).split_with_sizes(sizes)
     _call(_native.lib().tts_page_slots, device, *(_describe(n, t, device) for n, t in (("table", table), ("lengths", lengths), ("fresh", fresh), ("free", free), ("count", count))), page,
           *(_describe(n, t, device) for n, t in zip(("slots", "positions", "owners", "starts", "left"), made)))
     _written(table)
