@@ -180,15 +180,14 @@ __global__ __launch_bounds__(256, W > 4 ? 1 : ROWS < 16 ? 3 : 2) void kv4_attend
 
   // The rows, what they see, and q, on its way
   int low[RT], high[RT];  // [low, high)
-  bool live[RT];
   Dwords<4> raw[RT][W];
   for (int t = 0; t < RT; t++) {
     const int row = row0 + t * ROWS + m % ROWS, token = divided(row, p.by_group), head = kv * p.group + row - token * p.group;
-    live[t] = token < r.rows;
+    const bool live = token < r.rows;
     const int position = r.length - r.rows + token;
     low[t] = p.window ? max(position - p.window + 1, 0) : 0;
-    high[t] = live[t] ? min(position + 1, r.tokens) : 0;
-    const char *from = (const char *)p.q + 2 * ((int64_t)(r.first + (live[t] ? token : 0)) * p.q_token + (int64_t)head * p.q_head) + 16 * g * W;
+    high[t] = live ? min(position + 1, r.tokens) : 0;
+    const char *from = (const char *)p.q + 2 * ((int64_t)(r.first + (live ? token : 0)) * p.q_token + (int64_t)head * p.q_head) + 16 * g * W;
     for (int w = 0; w < W; w++) raw[t][w] = load_dwords<4>(from + 16 * w);
   }
 
@@ -256,18 +255,19 @@ __global__ __launch_bounds__(256, W > 4 ? 1 : ROWS < 16 ? 3 : 2) void kv4_attend
     float v[W][8], most = 0.f, sum = 0.f;
     for (int w = 0; w < W; w++)
       for (int e = 0; e < 8; e++) {
-        v[w][e] = live[t] ? half_of(raw[t][w].d[e / 2], BF16, e & 1) : 0.f;
+        v[w][e] = half_of(raw[t][w].d[e / 2], BF16, e & 1);  // (of a row that is not there: the first's, for nothing)
         most = fmaxf(most, fabsf(v[w][e])), sum += v[w][e];
       }
     most = over_row(most, [](float a, float b) { return fmaxf(a, b); });
     sum = over_row(sum, [](float a, float b) { return a + b; });
-    const float scaled = row_ops::fp16_scale(most), sign = p.scale < 0.f ? -scaled : p.scale == 0.f ? 0.f : scaled;
+    const int power_q = most > 0.f && most < __builtin_inff() ? max(-126, min(126, 14 - __builtin_amdgcn_frexp_expf(most))) : 0;
+    const float sign = __builtin_amdgcn_ldexpf(p.scale < 0.f ? -1.f : p.scale == 0.f ? 0.f : 1.f, power_q);
     for (int w = 0; w < W; w++) {
       float x[8];
       for (int e = 0; e < 8; e++) x[e] = v[w][e] * (e & 2 ? sign * 0x1p-4f : sign);
       q[t][w] = make_uint4(fp16_pair(x[0], x[1]), fp16_pair(x[2], x[3]), fp16_pair(x[4], x[5]), fp16_pair(x[6], x[7]));
     }
-    factor[t] = fmaxf(fabsf(p.scale) * LOG2_E * 0x1p24f / scaled, 0x1p-126f);
+    factor[t] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(p.scale) * LOG2_E, 24 - power_q), 0x1p-126f);
     // (a row with an infinity: NaN, as the formula gives, also where all its scores are -inf here)
     sum_q[t] = (sum - sum == 0.f ? sum : __builtin_nanf("")) * sign * 0x1p-24f;
   }
