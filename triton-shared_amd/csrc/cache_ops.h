@@ -82,7 +82,6 @@ struct AttendPlan {
   int64_t items;        // tiles of rows per head of the cache, at most
   int64_t extra;        // workgroups beyond one for each of them: slices of their tokens (0: none are sliced)
   float over_extra;     // 1 / extra
-  int round;            // a slice has a multiple of so many blocks of 64 tokens
 };
 
 struct AttendParams {

@@ -116,7 +116,7 @@ __device__ __forceinline__ Work work_of(const AttendParams &p, int index, int ro
     const float longest = over_lanes<16>((float)most, [](float a, float b) { return fmaxf(a, b); });
     // (rounded up past what 32 bits lose: no more slices than there are workgroups)
     const float each = fmaxf(all * p.plan.over_extra * 1.0001f, over_row(longest, [](float a, float b) { return fmaxf(a, b); }) * (1.0001f / MOST_SLICES));
-    size = ((int)fminf(each, 16777000.f) + 1 + p.plan.round - 1) & ~(p.plan.round - 1);
+    size = ((int)fminf(each, 16777000.f) + WAVES) / WAVES * WAVES;
   }
   Work w = {};
   int before = 0;
@@ -133,7 +133,7 @@ __device__ __forceinline__ Work work_of(const AttendParams &p, int index, int ro
       w.size = size * BLOCK;
       if (w.slices > 1) {  // slices of one length within the request
         const u32 blocks = (u32)get(r.blocks);
-        w.size = (int)(((blocks + w.slices - 1) / (u32)w.slices + p.plan.round - 1) & ~(p.plan.round - 1)) * BLOCK;
+        w.size = (int)(((blocks + w.slices - 1) / (u32)w.slices + WAVES - 1) / WAVES * WAVES) * BLOCK;
       }
       const int of = index - w.index;
       w.tile = index < 0 ? ((row - w.first) * p.group) >> tile_log : w.slices > 1 ? (int)((u32)of / (u32)w.slices) : of;
@@ -147,13 +147,14 @@ __device__ __forceinline__ Work work_of(const AttendParams &p, int index, int ro
   return w;
 }
 
-constexpr int most_row_tiles(int w) { return w <= 4 ? 2 : 1; }
+// of a wavefront that has rows of its own: what the registers of two wavefronts per SIMD hold
+constexpr int row_tiles_of(int w) { return w <= 4 ? 2 : 1; }
 
 // W: dim / 32.  RT: tiles of rows per wavefront, ROWS: of such a tile.  BY_ROWS: wavefronts have rows of their own; else all have the same rows, and blocks in turn.
 // The matrix instructions' tiles have 16 rows.  Of fewer (a token's heads of one key's) each is there 16 / ROWS times, and of the scores that a lane gets so, those of 4
 // tiles of tokens, it goes on with 4 ROWS / 16 of them: the copies share the softmax.
 template <bool BF16, int W, int RT, int ROWS, bool BY_ROWS>
-__global__ __launch_bounds__(256, W > 4 ? 1 : ROWS < 16 ? 3 : 2) void kv4_attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS == 16) ? 2 : 3) void kv4_attend_kernel(AttendParams p) {
   constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK, WAVE_ROWS = RT * ROWS, TILE = (BY_ROWS ? WAVES : 1) * WAVE_ROWS;
   constexpr int BANKS = 16 / ROWS, NJ = 4 / BANKS;
   constexpr int MEET_PITCH = D + 4, MEET_BYTES = BY_ROWS ? 0 : WAVES * WAVE_ROWS * (MEET_PITCH + 2) * 4;
@@ -513,12 +514,10 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
 template <bool BF16, int W>
 hipError_t launch_of(const AttendParams &p, hipStream_t s) {
   const dim3 grid((unsigned)((p.plan.items + p.plan.extra) * p.cache.heads + (p.clear ? 8 : 0)));
-  constexpr int MOST = most_row_tiles(W);
-  if (p.plan.by_rows) kv4_attend_kernel<BF16, W, MOST, 16, true><<<grid, 256, 0, s>>>(p);
+  if (p.plan.by_rows) kv4_attend_kernel<BF16, W, row_tiles_of(W), 16, true><<<grid, 256, 0, s>>>(p);
   else if (p.plan.tile_log == 2) kv4_attend_kernel<BF16, W, 1, 4, false><<<grid, 256, 0, s>>>(p);
   else if (p.plan.tile_log == 3) kv4_attend_kernel<BF16, W, 1, 8, false><<<grid, 256, 0, s>>>(p);
-  else if (p.plan.tile_log == 4) kv4_attend_kernel<BF16, W, 1, 16, false><<<grid, 256, 0, s>>>(p);
-  else kv4_attend_kernel<BF16, W, MOST, 16, false><<<grid, 256, 0, s>>>(p);
+  else kv4_attend_kernel<BF16, W, 1, 16, false><<<grid, 256, 0, s>>>(p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.plan.extra) {
     kv4_attend_join_kernel<BF16><<<dim3((unsigned)(p.tokens * p.heads)), 256, 0, s>>>(p);
@@ -543,22 +542,28 @@ hipError_t launch_as(const AttendParams &p, hipStream_t s) {
 
 }  // namespace
 
+// Which kernel, and how many workgroups.  Both sides of each rule as measured, us a call in a graph, dim 128 and 8 heads of the cache where nothing else is said:
+// * Rows of their own for each wavefront where a request has 128 and more on average and they make 384 workgroups: 64 requests of 256 rows 405 (shared rows 537), 16 of 512 217
+//   (267), but 16 of 256 166 (162) and 4 of 1024 140 (119): fewer workgroups do not fill the device, and the tokens are what is left to divide.
+// * Tiles of 4 or 8 rows where a request has no more: 16 requests of 4000 tokens, 4 rows 21.4 (tiles of 8 21.9, of 16 22.7), 8 rows 22.4 (of 16 23.3, of 4 30.6).
+// * Slices, of 512 workgroups beyond the tiles', where the longest request has more than 1024 tokens and 6 for each tile: 64 requests of up to 8192 36.2 (none: 50.7),
+//   128 of up to 8000 71.7 (76.1), one of 1500 11.7 (13.2), but 128 of 4000 120.9 (113.5), 256 of up to 2000 63.5 (41.4), one of 600 11.4 (9.3): the second kernel, and what a
+//   workgroup does before its first block and behind its last.
 AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, int dim, int64_t longest, int window) {
   AttendPlan plan = {};
   const int64_t group = heads / kv_heads, rows = (tokens + requests - 1) / std::max(requests, 1) * group;  // of a request, on average
-  plan.by_rows = rows > 64;
-  const int most = most_row_tiles(dim / 32) * 16;
-  const int tile = plan.by_rows ? WAVES * most : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : most;
-  plan.tile_log = __builtin_ctz(tile);
+  const int64_t wide = WAVES * 16 * row_tiles_of(dim / 32);
   // tiles: each request's rows rounded up, which is what they are where a token's rows fill whole tiles
-  plan.items = std::max<int64_t>(1, group % tile == 0 ? tokens * (group / tile) : (tokens * group + (int64_t)requests * (tile - 1)) / tile);
+  auto tiles = [&](int64_t tile) { return std::max<int64_t>(1, group % tile == 0 ? tokens * (group / tile) : (tokens * group + requests * (tile - 1)) / tile); };
+  plan.by_rows = rows >= 128 && tiles(wide) * kv_heads >= 384;
+  const int64_t tile = plan.by_rows ? wide : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  plan.tile_log = __builtin_ctzll(tile);
+  plan.items = tiles(tile);
   const int64_t range = window ? std::min<int64_t>(longest, (int64_t)window + tile / group + 17) : longest;
-  const int64_t wanted = plan.by_rows ? 256 : 512;
-  plan.round = plan.by_rows ? 1 : WAVES;
-  if (range > (plan.by_rows ? 4 : 1) * WAVES * BLOCK && (!plan.by_rows || plan.items * kv_heads < 256)) {
-    const int64_t most_extra = plan.items * std::min<int64_t>((range + BLOCK - 1) / BLOCK / plan.round, MOST_SLICES);  // (more than that has nothing to do)
-    plan.extra = std::max<int64_t>(0, std::min((wanted + kv_heads - 1) / kv_heads, most_extra));
-    plan.over_extra = plan.extra ? 1.f / (float)plan.extra : 0.f;
+  if (!plan.by_rows && range > 1024 && 6 * plan.items * kv_heads <= range) {
+    const int64_t most = plan.items * std::min<int64_t>((range + BLOCK - 1) / BLOCK / WAVES, MOST_SLICES);  // (more than that has nothing to do)
+    plan.extra = std::min((512 + kv_heads - 1) / (int64_t)kv_heads, most);
+    plan.over_extra = 1.f / (float)plan.extra;
   }
   return plan;
 }
