@@ -354,7 +354,7 @@ def check_rope(q, k, positions, cos_sin, w_q=None, w_k=None, eps=1e-6, interleav
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("T,Hq,Hk,D,R", [(1, 32, 8, 128, 128), (1, 1, 1, 2, 2), (3, 5, 1, 64, 64), (7, 4, 2, 96, 48), (5, 3, 3, 80, 40), (33, 6, 2, 80, 80), (9, 2, 1, 6, 4), (4, 3, 1, 50, 20), (2, 2, 1, 256, 64),
-                                         (5, 7, 1, 192, 192), (3, 2, 2, 512, 512), (2, 2, 1, 510, 256), (70, 15, 5, 128, 32), (13, 40, 8, 128, 128), (2, 1, 4, 144, 16)])
+                                         (5, 7, 1, 192, 192), (3, 2, 2, 512, 512), (2, 2, 1, 510, 256), (70, 15, 5, 128, 32), (13, 40, 8, 128, 128), (2, 1, 4, 144, 16), (5, 3, 1, 72, 24), (3, 2, 2, 200, 104), (2, 1, 1, 504, 8)])
 def test_rope(T, Hq, Hk, D, R, interleaved, dtype):
     q, k = gpu(T, Hq, D, seed=1, scale=3.0, dtype=dtype), gpu(T, Hk, D, seed=2, scale=0.2, dtype=dtype)
     g = torch.Generator(device="cuda")
@@ -611,18 +611,26 @@ def attend_exact(a, scale, window):
                 # the exponential: of a difference that is rounded, of a power of two within two steps
                 slip = torch.where(seen, off + 4 * U * (torch.where(seen, z, 0.0).abs() + most.abs()) + 6 * U, 0.0)
                 w = e / total.clamp(min=1e-300)
-                y = torch.zeros(f, D, dtype=torch.float64, device="cuda")
-                err = torch.zeros_like(y)
-                for r in range(f):  # (a NaN that a row does not see stays out of it)
-                    s = seen[r]
-                    if not bool(s.any()):
-                        continue
-                    wr, value, big = w[r, s], (cv * sv + lv)[s], (cv * sv)[s].abs() + lv[s].abs()
-                    y[r] = wr @ value
-                    count = int(s.sum())
-                    per = slip[r, s] + (count / 4 + 64) * 2 * U   # sums of as many tokens as a lane has, and joining them
-                    err[r] = (wr * (2 * per + (wr * per).sum())) @ big + 2.0 ** -11 * (wr @ (cv * sv)[s].abs())
-                    err[r] += 15 * count * 2.0 ** -34 * sv[s].abs().max() / total[r]
+                count = seen.sum(dim=1, keepdim=True).double()
+                # the sums: of as many tokens as a lane has, and joining them; the statistics' error, and that of each weight
+                per = torch.where(seen, slip + (count / 4 + 64) * 2 * U, 0.0)
+                value, big, codes = cv * sv + lv, (cv * sv).abs() + lv.abs(), (cv * sv).abs()
+                if bool(value.isfinite().all() and w.isfinite().all()):
+                    y = w @ value
+                    err = (w * (2 * per + (w * per).sum(dim=1, keepdim=True))) @ big + 2.0 ** -11 * (w @ codes)
+                    largest = torch.where(seen, sv.abs().t(), 0.0).amax(dim=1, keepdim=True)
+                    err = err + 15 * count * 2.0 ** -34 * largest / total.clamp(min=1e-300)
+                else:
+                    y = torch.zeros(f, D, dtype=torch.float64, device="cuda")
+                    err = torch.zeros_like(y)
+                    for r in range(f):  # (a NaN that a row does not see stays out of it)
+                        s = seen[r]
+                        if not bool(s.any()):
+                            continue
+                        wr, pr = w[r, s], per[r, s]
+                        y[r] = wr @ value[s]
+                        err[r] = (wr * (2 * pr + (wr * pr).sum())) @ big[s] + 2.0 ** -11 * (wr @ codes[s])
+                        err[r] += 15 * count[r] * 2.0 ** -34 * sv[s].abs().max() / total[r]
                 out[first:first + f, h], lim[first:first + f, h] = y, err + half(dtype) * (y.abs() + err) + smallest(dtype)
     return out, lim, real
 
@@ -667,6 +675,69 @@ def test_attend_in_slices(lengths, fresh, Hq, Hk, D, page):
         got = check_attend(wide, longest=longest)
         assert bool(((got.double() - first.double()).abs() <= 2 * (2.0 ** -8 * first.double().abs() + 0.01)).all())
     check_attend(wide, window=300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests,Hq,Hk", [(64, 4, 2), (65, 4, 2), (200, 4, 1), (130, 24, 2)])
+def test_attend_many_requests(requests, Hq, Hk):
+    rng = np.random.default_rng(requests)
+    lengths = rng.integers(0, 90, requests)
+    lengths[[3, requests - 2]] = 3500, 1300                                       # in slices, beside short ones
+    fresh = np.minimum(rng.integers(0, 4, requests), lengths)
+    a = make_attend(lengths.tolist(), fresh.tolist(), Hq, Hk, 64, 16, seed=requests)
+    check_attend(a)
+    check_attend(a, longest=1000)                                                 # ... in none
+    check_attend(a, window=40)
+
+
+@pytest.mark.gpu
+def test_attend_more_than_16_blocks_of_a_wavefront():
+    check_attend(make_attend([5000, 4200] + [10] * 14, [1] * 16, 64, 64, 32, 16, seed=1))
+
+
+@pytest.mark.gpu
+def test_attend_windows_that_see_everything():
+    a = make_attend([3, 300], [5, 40], 4, 2, 64)
+    want = check_attend(a)
+    for window in (301, 2 ** 30, 2 ** 31 - 1):
+        assert torch.equal(check_attend(a, window=window), want)
+
+
+# Calls of many rows in many workgroups: wavefronts with rows of their own
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_attend_many_rows(D, dtype):
+    a = make_attend([250, 391, 171], [240, 391, 150], 64, 64, D, 48, dtype, seed=D)
+    check_attend(a)
+    check_attend(a, window=65)
+
+
+@pytest.mark.gpu
+def test_attend_many_rows_of_shared_heads_and_what_is_not_there():
+    a = make_attend([260, 30, 401, 64, 0], [220, 30, 130, 5, 0], 192, 32, 64, 16, seed=3)
+    want = check_attend(a)
+    check_attend(a, window=1)
+    check_attend(a, window=130)
+    T = len(a["q"])
+    wide = gpu(T + 9, 200, 65, seed=4, dtype="bf16")
+    q = wide[:T, 3:195, 1:]
+    q.copy_(a["q"])
+    padded = a | dict(q=wide[:, 3:195, 1:])
+    assert torch.equal(check_attend(padded)[:T], want)
+    before = wide.clone()
+    assert torch.equal(check_attend(padded, out=padded["q"])[:T], want)          # in place, rows behind the last request as they were
+    wide[:T, 3:195, 1:] = before[:T, 3:195, 1:]
+    assert torch.equal(wide, before)
+    a["table"][0, 2], a["table"][2, 7], a["table"][2, 20] = -1, len(a["cache"]), 2 ** 31 - 1
+    check_attend(a)
+    k, v = a["k"].clone(), a["v"].clone()
+    v[int(a["table"][0, 15]) * 16 + 5, 3] = NAN                                   # position 245 of the first request, a head of the cache
+    k[int(a["table"][2, 19]) * 16 + 3, 7, 5] = -INF
+    check_attend(fill(a | dict(k=k, v=v), 16))
+    check_attend(fill(a | dict(k=k, v=v), 16), window=100)
+    long = make_attend([1500, 300], [130, 300], 96, 96, 64, 16, seed=5)
+    check_attend(long | dict(table=torch.nn.functional.pad(long["table"], (0, 500), value=-1)))
 
 
 @pytest.mark.gpu
@@ -949,7 +1020,8 @@ def test_steps_in_graphs():
 def test_results_do_not_change_from_call_to_call():
     a = make_attend([2000, 300, 77], [1, 1, 1], 8, 2, 128)
     b = make_attend([400, 300], [150, 120], 8, 2, 128)
-    for x in (a, b):
+    c = make_attend([250, 391, 171], [240, 391, 150], 64, 64, 64)
+    for x in (a, b, c):
         first = ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"])
         for _ in range(5):
             assert torch.equal(ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"]), first)

@@ -73,6 +73,9 @@ struct Work {
 // (starts are the caller's memory: whatever they hold, rows stay inside [0, tokens))
 __device__ __forceinline__ int start_of(const AttendParams &p, int b) { return (int)min((int64_t)max(p.starts[b], 0), p.tokens); }
 
+// at - by, at least 0 (`at` may be negative, and the difference none of 32 bits)
+__device__ __forceinline__ int behind(int at, int by) { return max(at, by) - by; }
+
 struct Request {
   int first, rows, length, tokens, begin, blocks, tiles;  // blocks: of 64 tokens, of what its rows see
 };
@@ -83,7 +86,7 @@ __device__ __forceinline__ Request request_of(const AttendParams &p, int b) {
   const int next = start_of(p, b + 1), length = p.lengths[b];
   r.rows = max(next - r.first, 0), r.length = max(length, 0);
   r.tokens = min(r.length, p.places);
-  r.begin = p.window ? max(r.length - r.rows + 1 - p.window, 0) & ~15 : 0;
+  r.begin = p.window ? behind(r.length - r.rows + 1, p.window) & ~15 : 0;
   r.blocks = (max(r.tokens - r.begin, 0) + BLOCK - 1) / BLOCK;
   r.tiles = (r.rows * p.group + (1 << p.plan.tile_log) - 1) >> p.plan.tile_log;
   return r;
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS =
     const int row = row0 + t * ROWS + m % ROWS, token = divided(row, p.by_group), head = kv * p.group + row - token * p.group;
     const bool live = token < r.rows;
     const int position = r.length - r.rows + token;
-    low[t] = p.window ? max(position - p.window + 1, 0) : 0;
+    low[t] = p.window ? behind(position, p.window - 1) : 0;
     high[t] = live ? min(position + 1, r.tokens) : 0;
     const char *from = (const char *)p.q + 2 * ((int64_t)(r.first + (live ? token : 0)) * p.q_token + (int64_t)head * p.q_head) + 16 * g * W;
     for (int w = 0; w < W; w++) raw[t][w] = load_dwords<4>(from + 16 * w);
@@ -195,11 +198,11 @@ __global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS =
   // all of a block's tokens are seen by all of the wavefront's rows where it lies inside [seen_from, seen_to)
   int seen_from, seen_to, last, window_begin;  // (the last two: where what any of them sees ends, and begins, at a multiple of 16)
   {
-    const int top = divided(row0, p.by_group), bottom = min(divided(row0 + WAVE_ROWS - 1, p.by_group), r.rows - 1), behind = r.length - r.rows + 1;
-    seen_from = p.window ? max(behind + bottom - p.window, 0) : 0;
-    seen_to = min(behind + top, r.tokens);
-    last = top < r.rows ? min(behind + bottom, r.tokens) : 0;
-    window_begin = p.window ? max(behind + top - p.window, 0) & ~15 : 0;
+    const int top = divided(row0, p.by_group), bottom = min(divided(row0 + WAVE_ROWS - 1, p.by_group), r.rows - 1), sees = r.length - r.rows + 1;  // (row 0: up to there)
+    seen_from = p.window ? behind(sees + bottom, p.window) : 0;
+    seen_to = min(sees + top, r.tokens);
+    last = top < r.rows ? min(sees + bottom, r.tokens) : 0;
+    window_begin = p.window ? behind(sees + top, p.window) & ~15 : 0;
   }
   const int slice_begin = r.begin + r.slice * r.size, end = __builtin_amdgcn_readfirstlane(min(slice_begin + r.size, last)), begin = max(slice_begin, window_begin);
   seen_from = __builtin_amdgcn_readfirstlane(seen_from), seen_to = __builtin_amdgcn_readfirstlane(min(seen_to, end));
@@ -560,7 +563,7 @@ AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, in
   plan.tile_log = __builtin_ctzll(tile);
   plan.items = tiles(tile);
   const int64_t range = window ? std::min<int64_t>(longest, (int64_t)window + tile / group + 17) : longest;
-  if (!plan.by_rows && range > 1024 && 6 * plan.items * kv_heads <= range) {
+  if (!plan.by_rows && range > 1024 && 6 * plan.items * kv_heads <= range && tokens * heads < (1 << 24)) {  // (as many workgroups join them, and a launch has less than 2^32 lanes)
     const int64_t most = plan.items * std::min<int64_t>((range + BLOCK - 1) / BLOCK / WAVES, MOST_SLICES);  // (more than that has nothing to do)
     plan.extra = std::min((512 + kv_heads - 1) / (int64_t)kv_heads, most);
     plan.over_extra = 1.f / (float)plan.extra;

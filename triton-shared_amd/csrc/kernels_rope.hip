@@ -112,6 +112,7 @@ hipError_t go(const RopeParams &p, hipStream_t s) {
   return hipSuccess;
 }
 
+// Units of 8 pairs where what is rotated and what is not are whole ones, of 4, or of one.
 template <class T, bool INTER>
 hipError_t launch_of(const RopeParams &p, hipStream_t s) {
   if (p.rotary % 16 == 0 && p.dim % 16 == 0) {
@@ -121,6 +122,7 @@ hipError_t launch_of(const RopeParams &p, hipStream_t s) {
     if (units <= 16) return go<T, 8, INTER, 16, 1, 1>(p, s);
     return go<T, 8, INTER, 32, 1, 1>(p, s);
   }
+  if (p.rotary % 8 == 0 && p.dim % 8 == 0) return p.dim <= 128 ? go<T, 4, INTER, 16, 1, 1>(p, s) : go<T, 4, INTER, 64, 1, 1>(p, s);
   return go<T, 1, INTER, 64, ROPE_MAX_DIM / 128, 1>(p, s);
 }
 

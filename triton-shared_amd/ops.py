@@ -19,6 +19,7 @@ Wrong arguments raise ValueError or TypeError, what is not implemented NotImplem
 They have no derivatives: tensors that require gradients are refused where gradients are recorded, and those with a forward-mode tangent anywhere.
 """
 import ctypes
+import math
 import operator
 
 import torch
@@ -318,6 +319,6 @@ def kv4_attention(q, cache, table, lengths, starts, scale=None, window=None, lon
     dq, dc, dt = _describe("q", q, device), _describe("cache", cache, device), _describe("table", table, device)
     work = _workspace(_native.lib().tts_kv4_attention_workspace, device, dq, dc, dt, window or 0, longest or 0)
     given, out = out, torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    _call(_native.lib().tts_kv4_attention, device, dq, dc, dt, _describe("lengths", lengths, device), _describe("starts", starts, device), float(q.shape[2] ** -0.5 if scale is None else scale),
+    _call(_native.lib().tts_kv4_attention, device, dq, dc, dt, _describe("lengths", lengths, device), _describe("starts", starts, device), float(1.0 / math.sqrt(q.shape[2]) if scale is None else scale),
           window or 0, longest or 0, given is None, _describe("out", out, device), work.data_ptr(), work.numel())
     return out if given is None else _written(out)
