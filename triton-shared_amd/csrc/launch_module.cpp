@@ -207,6 +207,38 @@ bool to_int64(PyObject *o, int64_t *out) {
   return !over;
 }
 
+// The DLPack standard's exchange interface of torch's tensors (version 1.x; a capsule on the type), of which one function is used: a tensor's description without
+// a reference to it, without a wait.  The layouts are the standard's.
+struct DLTensor {
+  void *data;
+  int32_t device_type, device_id;
+  int32_t ndim;
+  uint8_t code, bits;
+  uint16_t lanes;
+  int64_t *shape, *strides;
+  uint64_t byte_offset;
+};
+struct DLExchange {
+  uint32_t major, minor;
+  void *older, *allocate, *take, *give;
+  int (*describe)(void *object, DLTensor *out);
+};
+const DLExchange *g_exchange = nullptr;
+constexpr int DL_CUDA = 2, DL_ROCM = 10;
+
+// the tts_dtype of a DLPack type, or -1
+int dtype_of(const DLTensor &t) {
+  if (t.lanes != 1) return -1;
+  switch (t.code << 8 | t.bits) {
+    case 2 << 8 | 32: return TTS_F32;
+    case 2 << 8 | 16: return TTS_F16;
+    case 4 << 8 | 16: return TTS_BF16;
+    case 0 << 8 | 8: return TTS_I8;
+    case 0 << 8 | 32: return TTS_I32;
+    default: return -1;
+  }
+}
+
 // What a call knows of its tensors: they are all on the current device, and none wants a gradient.  `ok` false: not an ordinary call.
 struct Operands {
   int64_t device = -1;
@@ -229,6 +261,19 @@ struct Operands {
     if (o == Py_None || !ok) return nullptr;
     ok = false;
     if ((PyObject *)Py_TYPE(o) != g_tensor_type && (PyObject *)Py_TYPE(o) != g_parameter_type) return nullptr;
+    if (g_exchange) {
+      if (grad) {
+        Ref wants(PyObject_GetAttr(o, s_requires_grad));
+        if (wants.o != Py_False) return nullptr;
+      }
+      DLTensor d;
+      if (g_exchange->describe(o, &d) != 0 || (d.device_type != DL_ROCM && d.device_type != DL_CUDA) || d.device_id != device || d.ndim < 1 || d.ndim > 3 || !d.strides) return nullptr;
+      t.dtype = dtype_of(d), t.rank = d.ndim, t.ptr = (char *)d.data + d.byte_offset;
+      if (t.dtype < 0) return nullptr;
+      for (int i = 0; i < d.ndim; i++) t.shape[i] = d.shape[i], t.stride[i] = d.strides[i];
+      ok = true;
+      return &t;
+    }
     Ref on(PyObject_CallMethodNoArgs(o, s_get_device)), type(PyObject_GetAttr(o, s_dtype)), shape(PyObject_GetAttr(o, s_shape)), stride(PyObject_CallMethodNoArgs(o, s_stride)),
         ptr(PyObject_CallMethodNoArgs(o, s_data_ptr));
     int64_t index = -1;
@@ -498,6 +543,11 @@ PyObject *setup_ops(PyObject *, PyObject *args) {
   g_ops.attend_workspace = (decltype(g_ops.attend_workspace))(uintptr_t)f[9];
   g_ops.attend = (decltype(g_ops.attend))(uintptr_t)f[10];
   g_ops.route = (decltype(g_ops.route))(uintptr_t)f[0];
+  // without the interface (an older torch): by attributes
+  Ref capsule(PyObject_GetAttrString(g_tensor_type, "__dlpack_c_exchange_api__"));
+  const DLExchange *exchange = capsule && PyCapsule_CheckExact(capsule.o) ? (const DLExchange *)PyCapsule_GetPointer(capsule.o, "dlpack_exchange_api") : nullptr;
+  g_exchange = exchange && exchange->major == 1 && exchange->describe ? exchange : nullptr;
+  PyErr_Clear();
   Py_RETURN_NONE;
 }
 
