@@ -478,8 +478,11 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
   const int64_t first = (index * p.cache.heads + kv) * tile + (in_request & (tile - 1));
   const float *stats = p.stats + first * 2, *parts = p.parts + first * dim;
   const int four = dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64, at = tid % four, side = 256 / four;  // threads per slice, their element, slices at a time
-  f32x4 part = {0.f, 0.f, 0.f, 0.f};
-  if (tid / four < r.slices && 4 * at < dim) part = *(const f32x4 *)(parts + (tid / four) * part_step * dim + 4 * at);
+  const bool mine = 4 * at < dim;
+  // (the first four of a thread's on their way together, and the statistics with them)
+  f32x4 part[4];
+  for (int n = 0; n < 4; n++)
+    if (mine && tid / four + n * side < r.slices) part[n] = *(const f32x4 *)(parts + (tid / four + n * side) * part_step * dim + 4 * at);
   // (every wavefront for itself)
   float top[2], total[2], most = -__builtin_inff(), all = 0.f;
   for (int h = 0; h < 2; h++) {
@@ -497,15 +500,16 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
   all = over_lanes<64>(all, [](float a, float b) { return a + b; });
   __syncthreads();
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = tid / four; i < r.slices; i += side) {
-    f32x4 next = part;
-    if (i + side < r.slices && 4 * at < dim) next = *(const f32x4 *)(parts + (i + side) * part_step * dim + 4 * at);
-    for (int e = 0; e < 4; e++) sum[e] += part[e] * shares[i];
-    part = next;
+  for (int n = 0; n < 4; n++)
+    if (mine && tid / four + n * side < r.slices)
+      for (int e = 0; e < 4; e++) sum[e] += part[n][e] * shares[tid / four + n * side];
+  for (int i = tid / four + 4 * side; mine && i < r.slices; i += side) {
+    const f32x4 next = *(const f32x4 *)(parts + i * part_step * dim + 4 * at);
+    for (int e = 0; e < 4; e++) sum[e] += next[e] * shares[i];
   }
   sums[tid] = sum;
   __syncthreads();
-  if (tid >= four || 4 * at >= dim) return;
+  if (tid >= four || !mine) return;
   for (int i = 1; i < min(side, r.slices); i++)
     for (int e = 0; e < 4; e++) sum[e] += sums[tid + i * four][e];
   const float over = all == 0.f ? 0.f : 1.f / all;
