@@ -212,37 +212,43 @@ __global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS =
 
   const char *const cache = (const char *)p.cache.base + (int64_t)kv * p.cache.head_bytes;
   const int page = p.cache.page;
-  // the table's entries of 16 blocks: lane 4 n + j has that of tile j of block n
-  int entry = 0, within = 0;
+  // where the tiles of 16 blocks are in the cache: lane 4 n + j has tile j of block n
+  int64_t codes_at = 0, pairs_at = 0;
   unsigned long long there = 0;
   auto look_up = [&](int n) __attribute__((always_inline)) {
     const int token = start + (n + lane / 4) * STEP + lane % 4 * 16, column = divided(token, p.cache.by_page);
-    entry = -1;
+    int entry = -1;
     if (token < end) entry = p.table[(int64_t)r.request * p.ld_table + column];  // (end is inside the table)
     const bool ok = entry >= 0 && entry < p.cache.pages;
     there = __ballot(ok);
-    entry = ok ? entry : 0, within = token - column * page;
+    const int64_t begins = (ok ? entry : 0) * p.cache.page_bytes, within = token - column * page;
+    codes_at = begins + within * (D / 2), pairs_at = begins + within * 4;
+  };
+  auto from_lane = [&](int64_t v, int l) __attribute__((always_inline)) {
+    return (int64_t)((uint64_t)(u32)__builtin_amdgcn_readlane((int)((uint64_t)v >> 32), l) << 32 | (u32)__builtin_amdgcn_readlane((int)v, l));
   };
   // A block's keys, values and pairs.  Those of the next one are asked for as soon as the registers of this one's are free: values and pairs once they are in
   // LDS, keys behind their products.
   Dwords<W> keys[4], values[4];
   u32 key_pair, value_pair;
-  int64_t tiles[4];  // where they begin
+  const char *tiles[4];  // where they begin
   auto find = [&](int n) __attribute__((always_inline)) {
     if (n % 16 == 0) look_up(n);
-    for (int j = 0; j < 4; j++) {
-      const int at = n % 16 * 4 + j;
-      tiles[j] = (int64_t)__builtin_amdgcn_readlane(entry, at) * p.cache.page_bytes + (int64_t)__builtin_amdgcn_readlane(within, at) * (D / 2);
-    }
+    for (int j = 0; j < 4; j++) tiles[j] = cache + from_lane(codes_at, n % 16 * 4 + j);
   };
-  const char *const codes = cache + m * (D / 2) + g * (4 * W);
+  u32 mine_at = m * (D / 2) + g * (4 * W);
+  // (kept in 32 bits where it is used: a load takes a scalar address and an offset of that size)
+  auto from_tile = [&](const char *tile) __attribute__((always_inline)) {
+    asm("" : "+v"(mine_at));
+    return load_dwords<W>(tile + mine_at);
+  };
   auto load_keys = [&]() __attribute__((always_inline)) {
-    for (int j = 0; j < 4; j++) keys[j] = load_dwords<W>(codes + tiles[j]);
+    for (int j = 0; j < 4; j++) keys[j] = from_tile(tiles[j]);
   };
   auto load_values = [&](int n) __attribute__((always_inline)) {
-    for (int j = 0; j < 4; j++) values[j] = load_dwords<W>(codes + (int64_t)page * (D / 2) + tiles[j]);
+    for (int j = 0; j < 4; j++) values[j] = from_tile(tiles[j] + (int64_t)page * (D / 2));
     const int at = n % 16 * 4 + g, token = start + n * STEP + lane;
-    const char *pairs = cache + (int64_t)__shfl(entry, at) * p.cache.page_bytes + (int64_t)page * D + (__shfl(within, at) + m) * 4;
+    const char *pairs = cache + (int64_t)page * D + __shfl(pairs_at, at) + m * 4;
     key_pair = *(const u32 *)pairs, value_pair = *(const u32 *)(pairs + page * 4);
     if (token >= end || !(there >> at & 1)) key_pair = value_pair = 0;  // (memory that was never written may hold any)
   };
