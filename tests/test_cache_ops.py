@@ -601,8 +601,9 @@ def attend_exact(a, scale, window):
                 x = q[first:first + f, h].double()
                 z = (x @ (ck * sk + lk).t()) * scale
                 size = (x.abs() @ ck.t() * sk.t().abs() + x.abs().sum(dim=1, keepdim=True) * lk.t().abs()) * abs(scale)
-                # the score: D products and as many sums of each part, of which a sum may be cut where it is not rounded, four factors, and q's elements below 2^-35 of the largest
-                off = (2 * D + 20) * U * size + 2.0 ** -35 * x.abs().amax(dim=1, keepdim=True) * (ck.sum(dim=1)[None] * sk.t().abs()) * abs(scale)
+                # the score: D products and as many sums of each part, of which a sum may be cut where it is not rounded, four factors, and q: fp16's last place below its normal
+                # numbers, 2^-24, of which half is lost, times 16 for half of the elements, where the largest is 2^13 at least: 2^-34 of that
+                off = (2 * D + 20) * U * size + 2.0 ** -34 * x.abs().amax(dim=1, keepdim=True) * (ck.sum(dim=1)[None] * sk.t().abs()) * abs(scale)
                 z = torch.where(seen, z, -INF)
                 most = z.amax(dim=1, keepdim=True)
                 most = torch.where(most == -INF, 0.0, most)

@@ -48,7 +48,7 @@ struct RopeParams {
   float eps;
   int elem;             // ElemKind of q and k
   int w_f32, interleaved, clear;
-  FastDiv by_chunks;    // of a token's heads (the launch's own)
+  FastDiv by_all_heads; // (the launch's own)
 };
 hipError_t launch_rope(const RopeParams &p, hipStream_t s);
 

@@ -1,6 +1,10 @@
 // The paged cache held in 4 bits, written and read.  Of a token's head, for keys and values each:
 //   lowest = min(x),  step = (max(x) - min(x)) / 15 in 32 bits, rounded to the type,  code = how many of the borders (n + 1/2) step, n = 0 .. 14, x - lowest is above;
 // what it then stands for is code * step + lowest.  A head whose range is not finite in 32 bits (it holds a NaN or an infinity) gets a step of NaN.
+// The 16 bits of step and lowest value are the format's: lowest is an element, exactly, and the rounding of step moves what the highest code stands for by 15 / 2 of a step's last place,
+// a thirtieth of a step in bf16.
+// What bounds them, 16384 tokens of 8 heads of 128: writing 23.8 us, 3.5 TB/s, by some 17 instructions an element; reading 19.5 us, 4.3 TB/s, by memory (at a copy's rate
+// 17 each).  64 tokens: 3.0 and 2.4 us, a launch.
 #include <algorithm>
 
 #include "cache_ops.h"

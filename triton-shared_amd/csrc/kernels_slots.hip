@@ -43,7 +43,8 @@ __device__ __forceinline__ int last_begun(const int *begins, int n, int at) {
 }
 
 // Every workgroup adds up all requests' rows and pages for itself (a few KB from L2, and no second launch), then takes its share of the
-// rows and of the pages.
+// rows and of the pages; a row finds its request by halving in LDS.
+// What bounds it: a launch and a chain of loads (lengths, then the table or the stack).  64 requests of a token each 4.0 us, 211 with 3742 rows 5.0.
 __global__ __launch_bounds__(THREADS) void page_slots_kernel(SlotsParams p) {
   extern __shared__ int begins[];  // of the requests' rows, and of their new pages
   __shared__ Sums waves[THREADS / 64];
