@@ -704,6 +704,34 @@ def test_attend_windows_that_see_everything():
         assert torch.equal(check_attend(a, window=window), want)
 
 
+# Calls of many short requests: wavefronts with heads of their own (also where `longest` is not true)
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_attend_many_short_requests(D, dtype):
+    a = make_attend([70, 300, 1, 0, 129, 64, 17, 1090], [1, 1, 1, 0, 3, 2, 1, 1], 64, 64, D, 16, dtype, seed=D)
+    check_attend(a, longest=100)
+    check_attend(a, longest=100, window=65)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests,Hq,Hk,fresh", [(60, 20, 5, 1), (40, 48, 6, 3), (60, 35, 7, 2), (80, 4, 4, 4)])
+def test_attend_many_short_requests_of_shared_heads(requests, Hq, Hk, fresh):
+    rng = np.random.default_rng(requests + Hk)
+    lengths = rng.integers(0, 130, requests)
+    new = np.minimum(rng.integers(0, fresh + 1, requests), lengths)
+    a = make_attend(lengths.tolist(), new.tolist(), Hq, Hk, 64, 16, seed=requests)
+    check_attend(a, longest=60)
+    padded = a | dict(q=torch.cat([a["q"], gpu(6, Hq, 64, seed=50, dtype="bf16")]))
+    check_attend(padded, longest=60)
+    check_attend(padded, longest=60, out=torch.full_like(padded["q"], 5.0))
+    a["table"][::3, 1:3], a["table"][1::7, 0] = -1, len(a["cache"])
+    check_attend(a, longest=60)
+    v = a["v"].clone()
+    v[::5, 1] = NAN
+    check_attend(fill(a | dict(v=v), 16), longest=60)
+
+
 # Calls of many rows in many workgroups: wavefronts with rows of their own
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
@@ -1021,8 +1049,9 @@ def test_steps_in_graphs():
 def test_results_do_not_change_from_call_to_call():
     a = make_attend([2000, 300, 77], [1, 1, 1], 8, 2, 128)
     b = make_attend([400, 300], [150, 120], 8, 2, 128)
-    c = make_attend([250, 391, 171], [240, 391, 150], 64, 64, 64)
-    for x in (a, b, c):
-        first = ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"])
+    c, d = make_attend([250, 391, 171], [240, 391, 150], 64, 64, 64), make_attend([70, 300, 1, 129] * 3, [1] * 12, 64, 64, 64)
+    for x in (a, b, c, d):
+        call = lambda: ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"], longest=100 if x is d else None)  # noqa: E731, B023
+        first = call()
         for _ in range(5):
-            assert torch.equal(ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"]), first)
+            assert torch.equal(call(), first)

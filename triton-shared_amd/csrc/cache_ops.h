@@ -76,8 +76,9 @@ hipError_t launch_kv4_write(const Kv4RowsParams &p, hipStream_t s);
 hipError_t launch_kv4_read(const Kv4RowsParams &p, hipStream_t s);
 
 // How a call's rows and lengths are dealt to workgroups (kernels_kv4_attend.hip)
+enum AttendOwn { OWN_BLOCKS = 0, OWN_ROWS = 1, OWN_HEADS = 2 };
 struct AttendPlan {
-  int by_rows;          // the four wavefronts have rows of their own (else a share of the tokens each)
+  int own;              // AttendOwn: what a workgroup's four wavefronts have of their own
   int tile_log;         // log2 of a workgroup's rows
   int64_t items;        // tiles of rows per head of the cache, at most
   int64_t extra;        // workgroups beyond one for each of them: slices of their tokens (0: none are sliced)
@@ -94,7 +95,7 @@ struct AttendParams {
   int64_t q_token, q_head, o_token, o_head, ld_table, tokens;
   int requests, heads, group;
   int places;           // tokens that a request's row of the table has places for
-  FastDiv by_group, by_heads, by_kv_heads;
+  FastDiv by_group, by_heads, by_per_item;  // (the last: workgroups per tile or slice, the launch's own)
   int window;           // 0: none
   int clear;            // rows of no request get zeros
   float scale;

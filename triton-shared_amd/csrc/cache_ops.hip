@@ -67,7 +67,7 @@ struct Attend {
     if (p.requests > (1 << 20)) unsupported("table: " + std::to_string(p.requests) + " requests");
     const int64_t most = std::min(table.size(1) * p.cache.page, (int64_t)INT_MAX / 2);
     p.places = (int)most;
-    p.by_group = fast_div(p.group), p.by_heads = fast_div(p.heads), p.by_kv_heads = fast_div(p.cache.heads);
+    p.by_group = fast_div(p.group), p.by_heads = fast_div(p.heads);
     p.plan = plan_attend(p.tokens, p.requests, p.heads, p.cache.heads, p.cache.dim, longest ? std::min(longest, most) : most, window);
     // (a launch of 2^32 lanes and more starts only their remainder)
     if ((p.plan.items + p.plan.extra) * p.cache.heads >= (1 << 24)) unsupported(std::to_string(p.requests) + " requests of " + std::to_string(p.cache.heads) + " heads: more workgroups than a launch has");

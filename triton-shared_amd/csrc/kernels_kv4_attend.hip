@@ -160,17 +160,17 @@ __device__ __forceinline__ Work work_of(const AttendParams &p, int index, int ro
 // of a wavefront that has rows of its own: what the registers of two wavefronts per SIMD hold
 constexpr int row_tiles_of(int w) { return w <= 4 ? 2 : 1; }
 
-// W: dim / 32.  RT: tiles of rows per wavefront, ROWS: of such a tile.  BY_ROWS: wavefronts have rows of their own; else all have the same rows, and blocks in turn.
+// W: dim / 32.  RT: tiles of rows per wavefront, ROWS: of such a tile.  OWN: what of a workgroup's wavefronts have of their own: blocks of tokens, in turn; rows; heads of the cache.
 // The matrix instructions' tiles have 16 rows.  Of fewer (a token's heads of one key's) each is there 16 / ROWS times, and of the scores that a lane gets so, those of 4
 // tiles of tokens, it goes on with 4 ROWS / 16 of them: the copies share the softmax.
-template <bool BF16, int W, int RT, int ROWS, bool BY_ROWS>
-__global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS == 16) ? 2 : 3) void kv4_attend_kernel(AttendParams p) {
-  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK, WAVE_ROWS = RT * ROWS, TILE = (BY_ROWS ? WAVES : 1) * WAVE_ROWS;
+template <bool BF16, int W, int RT, int ROWS, int OWN>
+__global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 && ROWS == 16) ? 2 : 3) void kv4_attend_kernel(AttendParams p) {
+  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK, WAVE_ROWS = RT * ROWS, TILE = (OWN == OWN_ROWS ? WAVES : 1) * WAVE_ROWS;
   constexpr int BANKS = 16 / ROWS, NJ = 4 / BANKS;
-  constexpr int MEET_PITCH = D + 4, MEET_BYTES = BY_ROWS ? 0 : WAVES * WAVE_ROWS * (MEET_PITCH + 2) * 4;
+  constexpr int MEET_PITCH = D + 4, MEET_BYTES = OWN != OWN_BLOCKS ? 0 : WAVES * WAVE_ROWS * (MEET_PITCH + 2) * 4;
   __shared__ __attribute__((aligned(16))) char lds[MEET_BYTES > WAVES * WAVE_BYTES ? MEET_BYTES : WAVES * WAVE_BYTES];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), m = lane % 16, g = lane / 16, bank = m / ROWS;
-  const int kv_heads = p.cache.heads, groups = (int)(p.plan.items + p.plan.extra) * kv_heads;
+  const int kv_heads = p.cache.heads, per_item = OWN == OWN_HEADS ? (kv_heads + WAVES - 1) / WAVES : kv_heads, groups = (int)(p.plan.items + p.plan.extra) * per_item;
 
   if ((int)blockIdx.x >= groups) {  // rows of no request
     const int64_t from = p.requests ? start_of(p, 0) : 0, to = max(from, p.requests ? (int64_t)start_of(p, p.requests) : 0), others = from + p.tokens - to, size = (int64_t)p.heads * D;
@@ -181,13 +181,14 @@ __global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS =
     return;
   }
   // (the last first: of a prompt's tiles those have the most tokens)
-  const int item = (int)(p.plan.items + p.plan.extra) - 1 - divided(blockIdx.x, p.by_kv_heads), kv = blockIdx.x - (int)(p.plan.items + p.plan.extra - 1 - item) * kv_heads;
+  const int behind_it = divided(blockIdx.x, p.by_per_item), item = (int)(p.plan.items + p.plan.extra) - 1 - behind_it;
+  const int kv = OWN == OWN_HEADS ? (int)(blockIdx.x - behind_it * per_item) * WAVES + wave : blockIdx.x - behind_it * per_item;
   const Work r = work_of(p, item, 0);
-  if (!r.rows) return;
+  if (!r.rows || (OWN == OWN_HEADS && kv >= kv_heads)) return;
 
   char *const mine = lds + wave * WAVE_BYTES;
   float *const key_step = (float *)(mine + V_BYTES), *const key_low = key_step + BLOCK, *const value_step = key_low + BLOCK, *const value_low = value_step + BLOCK;
-  const int row0 = r.tile * TILE + (BY_ROWS ? wave * WAVE_ROWS : 0);  // of the request's tokens and the group's heads
+  const int row0 = r.tile * TILE + (OWN == OWN_ROWS ? wave * WAVE_ROWS : 0);  // of the request's tokens and the group's heads
 
   // The rows, what they see, and q, on its way
   int low[RT], high[RT];  // [low, high)
@@ -213,8 +214,8 @@ __global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS =
   }
   const int slice_begin = r.begin + r.slice * r.size, end = __builtin_amdgcn_readfirstlane(min(slice_begin + r.size, last)), begin = max(slice_begin, window_begin);
   seen_from = __builtin_amdgcn_readfirstlane(seen_from), seen_to = __builtin_amdgcn_readfirstlane(min(seen_to, end));
-  constexpr int STEP = BY_ROWS ? BLOCK : WAVES * BLOCK;
-  const int start = __builtin_amdgcn_readfirstlane(begin + (BY_ROWS ? 0 : wave * BLOCK));
+  constexpr int STEP = OWN != OWN_BLOCKS ? BLOCK : WAVES * BLOCK;
+  const int start = __builtin_amdgcn_readfirstlane(begin + (OWN != OWN_BLOCKS ? 0 : wave * BLOCK));
   const int blocks = __builtin_amdgcn_readfirstlane(end > start ? (end - start + STEP - 1) / STEP : 0);
 
   const char *const cache = (const char *)p.cache.base + (int64_t)kv * p.cache.head_bytes;
@@ -445,9 +446,10 @@ __global__ __launch_bounds__(256, W > 4 || BY_ROWS || (!BF16 && W == 4 && ROWS =
       if (element == 0) p.stats[part * 2] = most, p.stats[part * 2 + 1] = sum;
     }
   };
-  if constexpr (BY_ROWS) {
-    for (int t = 0; t < RT; t++)
-      for (int d = 0; d < D / 16; d++) put(wave * WAVE_ROWS + t * 16 + m, 16 * d + 4 * g, out[d][t], top[t], total[t]);
+  if constexpr (OWN != OWN_BLOCKS) {
+    if (bank == 0)
+      for (int t = 0; t < RT; t++)
+        for (int d = 0; d < D / 16; d++) put(row0 - tile0 + t * ROWS + m, 16 * d + 4 * g, out[d][t], top[t], total[t]);
   } else {  // the wavefronts' parts meet in LDS
     float *const rows = (float *)lds, *const tops = rows + WAVES * WAVE_ROWS * MEET_PITCH, *const totals = tops + WAVES * WAVE_ROWS;
     __syncthreads();
@@ -533,11 +535,19 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
 
 template <bool BF16, int W>
 hipError_t launch_of(const AttendParams &p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.plan.items + p.plan.extra) * p.cache.heads + (p.clear ? 8 : 0)));
-  if (p.plan.by_rows) kv4_attend_kernel<BF16, W, row_tiles_of(W), 16, true><<<grid, 256, 0, s>>>(p);
-  else if (p.plan.tile_log == 2) kv4_attend_kernel<BF16, W, 1, 4, false><<<grid, 256, 0, s>>>(p);
-  else if (p.plan.tile_log == 3) kv4_attend_kernel<BF16, W, 1, 8, false><<<grid, 256, 0, s>>>(p);
-  else kv4_attend_kernel<BF16, W, 1, 16, false><<<grid, 256, 0, s>>>(p);
+  const int per_item = p.plan.own == OWN_HEADS ? (p.cache.heads + WAVES - 1) / WAVES : p.cache.heads;
+  AttendParams q = p;
+  q.by_per_item = fast_div(per_item);
+  const dim3 grid((unsigned)((p.plan.items + p.plan.extra) * per_item + (p.clear ? 8 : 0)));
+  auto go = [&](auto rows) __attribute__((always_inline)) {
+    constexpr int ROWS = decltype(rows)::value;
+    if (p.plan.own == OWN_HEADS) kv4_attend_kernel<BF16, W, 1, ROWS, OWN_HEADS><<<grid, 256, 0, s>>>(q);
+    else kv4_attend_kernel<BF16, W, 1, ROWS, OWN_BLOCKS><<<grid, 256, 0, s>>>(q);
+  };
+  if (p.plan.own == OWN_ROWS) kv4_attend_kernel<BF16, W, row_tiles_of(W), 16, OWN_ROWS><<<grid, 256, 0, s>>>(q);
+  else if (p.plan.tile_log == 2) go(row_ops::Int<4>{});
+  else if (p.plan.tile_log == 3) go(row_ops::Int<8>{});
+  else go(row_ops::Int<16>{});
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.plan.extra) {
     kv4_attend_join_kernel<BF16><<<dim3((unsigned)(p.tokens * p.heads)), 256, 0, s>>>(p);
@@ -565,6 +575,9 @@ hipError_t launch_as(const AttendParams &p, hipStream_t s) {
 // Which kernel, and how many workgroups.  Both sides of each rule as measured, us a call in a graph, dim 128 and 8 heads of the cache where nothing else is said:
 // * Rows of their own for each wavefront where a request has 128 and more on average and they make 384 workgroups: 64 requests of 256 rows 405 (shared rows 537), 16 of 512 217
 //   (267), but 16 of 256 166 (162) and 4 of 1024 140 (119): fewer workgroups do not fill the device, and the tokens are what is left to divide.
+// * Heads of their own for each wavefront where there are 4 requests and heads for each token of the longest: 256 requests of 250 17.4 (shared blocks 27.1), 128 of up to 60 7.4 (12.6),
+//   512 of up to 1000 45.5 (58.9), but 64 of up to 250 10.4 (8.3), 128 of up to 1000 25.4 (19.0); between them 256 of up to 1000 27.8 (29.0): what a workgroup does before and after
+//   its blocks counts for four heads, and a head's blocks come one after another.
 // * Tiles of 4 or 8 rows where a request has no more: 16 requests of 4000 tokens, 4 rows 21.4 (tiles of 8 21.9, of 16 22.7), 8 rows 22.4 (of 16 23.3, of 4 30.6).
 // * Slices, of 512 workgroups beyond the tiles', where the longest request has more than 1024 tokens and 6 for each tile: 64 requests of up to 8192 36.2 (none: 50.7),
 //   128 of up to 8000 71.7 (76.1), one of 1500 11.7 (13.2), but 128 of 4000 120.9 (113.5), 256 of up to 2000 63.5 (41.4), one of 600 11.4 (9.3): the second kernel, and what a
@@ -575,12 +588,13 @@ AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, in
   const int64_t wide = WAVES * 16 * row_tiles_of(dim / 32);
   // tiles: each request's rows rounded up, which is what they are where a token's rows fill whole tiles
   auto tiles = [&](int64_t tile) { return std::max<int64_t>(1, group % tile == 0 ? tokens * (group / tile) : (tokens * group + requests * (tile - 1)) / tile); };
-  plan.by_rows = rows >= 128 && tiles(wide) * kv_heads >= 384;
-  const int64_t tile = plan.by_rows ? wide : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  const bool by_rows = rows >= 128 && tiles(wide) * kv_heads >= 384;
+  const int64_t tile = by_rows ? wide : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
   plan.tile_log = __builtin_ctzll(tile);
   plan.items = tiles(tile);
   const int64_t range = window ? std::min<int64_t>(longest, (int64_t)window + tile / group + 17) : longest;
-  if (!plan.by_rows && range > 1024 && 6 * plan.items * kv_heads <= range && tokens * heads < (1 << 24)) {  // (as many workgroups join them, and a launch has less than 2^32 lanes)
+  plan.own = by_rows ? OWN_ROWS : kv_heads >= WAVES && 4 * range <= plan.items * kv_heads ? OWN_HEADS : OWN_BLOCKS;
+  if (plan.own == OWN_BLOCKS && range > 1024 && 6 * plan.items * kv_heads <= range && tokens * heads < (1 << 24)) {  // (as many workgroups join them, and a launch has less than 2^32 lanes)
     const int64_t most = plan.items * std::min<int64_t>((range + BLOCK - 1) / BLOCK / WAVES, MOST_SLICES);  // (more than that has nothing to do)
     plan.extra = std::min((512 + kv_heads - 1) / (int64_t)kv_heads, most);
     plan.over_extra = 1.f / (float)plan.extra;
