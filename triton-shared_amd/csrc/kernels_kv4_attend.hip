@@ -477,13 +477,14 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
   }
 }
 
-// The slices of a row, where there are several, added up in their order: a workgroup per row, four elements a thread and as many slices side by side as that leaves.
-template <bool BF16>
+// The slices of a row, where there are several, added up in their order by TPR threads: four elements a thread, and as many slices side by side as that leaves.
+template <bool BF16, int TPR>
 __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
-  __shared__ float shares[MOST_SLICES];
+  __shared__ float shares_of[256 / TPR][MOST_SLICES];
   __shared__ f32x4 sums[256];
-  const int tid = threadIdx.x, lane = tid % 64, dim = p.cache.dim;
-  const int token = divided(blockIdx.x, p.by_heads), head = blockIdx.x - token * p.heads;
+  const int tid = threadIdx.x % TPR, lane = threadIdx.x % 64, dim = p.cache.dim, row = blockIdx.x * (256 / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  const int token = divided(row, p.by_heads), head = row - token * p.heads;
+  if (token >= p.tokens) return;
   const Work r = work_of(p, -1, token);
   if (!r.rows || r.slices == 1) return;  // a row of no request, or written already
   const int kv = divided(head, p.by_group), in_request = (token - r.first) * p.group + head - kv * p.group, tile = 1 << p.plan.tile_log;
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
   if (index + r.slices > p.plan.items + p.plan.extra) return;  // (only where starts are not in order)
   const int64_t first = (index * p.cache.heads + kv) * tile + (in_request & (tile - 1));
   const float *stats = p.stats + first * 2, *parts = p.parts + first * dim;
-  const int four = dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64, at = tid % four, side = 256 / four;  // threads per slice, their element, slices at a time
+  const int four = dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64, at = tid % four, side = TPR / four;  // threads per slice, their element, slices at a time
   const bool mine = 4 * at < dim;
   // (the first four of a thread's on their way together, and the statistics with them)
   f32x4 part[4];
@@ -507,13 +508,21 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
   }
   most = over_lanes<64>(most, [](float a, float b) { return fmaxf(a, b); });
   const float base = most == -__builtin_inff() ? 0.f : most;
+  float *shares = shares_of[threadIdx.x / TPR];
   for (int h = 0; h < 2; h++) {
     const float share = __builtin_amdgcn_exp2f(top[h] - base);
     all += total[h] * share;
     if (tid < 64) shares[lane + 64 * h] = share;
   }
   all = over_lanes<64>(all, [](float a, float b) { return a + b; });
-  __syncthreads();
+  auto meet = [&]() __attribute__((always_inline)) {
+    if constexpr (TPR > 64) __syncthreads();
+    else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  meet();
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   for (int n = 0; n < 4; n++)
     if (mine && tid / four + n * side < r.slices)
@@ -522,11 +531,11 @@ __global__ __launch_bounds__(256) void kv4_attend_join_kernel(AttendParams p) {
     const f32x4 next = *(const f32x4 *)(parts + i * part_step * dim + 4 * at);
     for (int e = 0; e < 4; e++) sum[e] += next[e] * shares[i];
   }
-  sums[tid] = sum;
-  __syncthreads();
+  sums[threadIdx.x] = sum;
+  meet();
   if (tid >= four || !mine) return;
   for (int i = 1; i < min(side, r.slices); i++)
-    for (int e = 0; e < 4; e++) sum[e] += sums[tid + i * four][e];
+    for (int e = 0; e < 4; e++) sum[e] += sums[threadIdx.x + i * four][e];
   const float over = all == 0.f ? 0.f : 1.f / all;
   uint16_t out[4];
   for (int e = 0; e < 4; e++) out[e] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)(sum[e] * over)) : __builtin_bit_cast(uint16_t, (_Float16)(sum[e] * over));
@@ -550,7 +559,10 @@ hipError_t launch_of(const AttendParams &p, hipStream_t s) {
   else go(row_ops::Int<16>{});
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.plan.extra) {
-    kv4_attend_join_kernel<BF16><<<dim3((unsigned)(p.tokens * p.heads)), 256, 0, s>>>(p);
+    const unsigned rows = (unsigned)(p.tokens * p.heads);
+    // (64 ragged requests of 32 heads 34.5 us in all, with 256 threads a row 35.9; 2 requests of 64 heads 42.6 and 37.0)
+    if (rows >= 1024) kv4_attend_join_kernel<BF16, 64><<<dim3((rows + 3) / 4), 256, 0, s>>>(p);
+    else kv4_attend_join_kernel<BF16, 256><<<dim3(rows), 256, 0, s>>>(p);
     e = hipGetLastError();
   }
   return e;
