@@ -13,7 +13,7 @@
 // operand of  out[element][row]  as it stands.  Its left operand, 16 tokens of one element per lane, is read out of LDS by ds_read_b64_tr_b4.
 //
 // What bounds it, dim 128 and 8 heads of the cache, bf16 (a copy of 1 GiB runs at 5.0 TB/s, a 16-bit matrix product of 8192^3 at 1.19 PFLOP/s):
-//   64 requests of 100 .. 8192 tokens (118 MB): 36 us in a graph, of which joining the slices 5: 3.8 TB/s while it runs.  The chain before a workgroup's first block, 3.4 us where it is alone
+//   64 requests of 100 .. 8192 tokens (118 MB): 35 us in a graph, of which joining the slices 4: 3.8 TB/s while it runs.  The chain before a workgroup's first block, 3.4 us where it is alone
 //     (lengths, table and codes, one after another), and its last steps are not hidden by others: there is one round of workgroups, and more of them cost as much as they hide.
 //   2 of 131072, 64 heads of q: 35 us, 29 + 6: 4.4 TB/s.   1 of 4000: 11.4 us, 8.3 + 3.2: the chains.
 //   4 x 1024 rows behind up to 4096 tokens: 219 us, 602 TFLOP/s: the vector instructions, some 570 to 64 matrix instructions in a block of 32 rows (160 of them unpack codes, 350 are the softmax); they
@@ -591,7 +591,7 @@ hipError_t launch_as(const AttendParams &p, hipStream_t s) {
 //   512 of up to 1000 45.5 (58.9), but 64 of up to 250 10.4 (8.3), 128 of up to 1000 25.4 (19.0); between them 256 of up to 1000 27.8 (29.0): what a workgroup does before and after
 //   its blocks counts for four heads, and a head's blocks come one after another.
 // * Tiles of 4 or 8 rows where a request has no more: 16 requests of 4000 tokens, 4 rows 21.4 (tiles of 8 21.9, of 16 22.7), 8 rows 22.4 (of 16 23.3, of 4 30.6).
-// * Slices, of 512 workgroups beyond the tiles', where the longest request has more than 1024 tokens and 6 for each tile: 64 requests of up to 8192 36.2 (none: 50.7),
+// * Slices, of 512 workgroups beyond the tiles', where the longest request has more than 1024 tokens and 6 for each tile: 64 requests of up to 8192 34.8 (none: 50.7),
 //   128 of up to 8000 71.7 (76.1), one of 1500 11.7 (13.2), but 128 of 4000 120.9 (113.5), 256 of up to 2000 63.5 (41.4), one of 600 11.4 (9.3): the second kernel, and what a
 //   workgroup does before its first block and behind its last.
 AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, int dim, int64_t longest, int window) {

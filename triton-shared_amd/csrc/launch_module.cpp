@@ -170,7 +170,7 @@ PyObject *setup(PyObject *, PyObject *args) {
 // Each function below is the ordinary call of the function of its name in ops.py -- torch tensors on the current device, no gradients; inside a level
 // of forward-mode derivatives ops.py does not come here -- and returns its result; for anything else it returns None before anything has
 // happened, and ops.py does the call or raises.
-// Host time of a call, in Python and ctypes -> here (us): moe_route 15.0 -> 9.4, moe_experts 27.4 -> 17.8, lora_add 21.8 -> 13.2 (one, three and
+// Host time of a call, in Python and ctypes -> here (us): moe_route 15.0 -> 7.3, moe_experts 27.4 -> 18 (of which the device is as long), lora_add 21.8 -> 10.8 (one, three and
 // two launches among them).
 struct Ops {
   decltype(&tts_moe_route) route;
