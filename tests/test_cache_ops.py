@@ -704,6 +704,16 @@ def test_attend_windows_that_see_everything():
         assert torch.equal(check_attend(a, window=window), want)
 
 
+# (what a window leaves of a length near 2^31 begins where 32 bits end)
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hk,fresh,longest", [(4, 2, 1, None), (4, 2, 6, None), (64, 64, 1, 100), (64, 64, 130, None)])
+def test_attend_windows_of_lengths_far_past_the_table(Hq, Hk, fresh, longest):
+    a = make_attend([640, 704, 1296, 656], [fresh] * 4, Hq, Hk, 64)
+    a["lengths"] = ints([2 ** 31 - 1, 2 ** 31 - 90, 1296, 2 ** 31 - 400])
+    for window in (1, 17, 65, 300, 2 ** 30, 2 ** 31 - 1):
+        check_attend(a, window=window, longest=longest)
+
+
 # Calls of many short requests: wavefronts with heads of their own (also where `longest` is not true)
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])

@@ -93,7 +93,7 @@ __device__ __forceinline__ Request request_of(const AttendParams &p, int b) {
   const int next = start_of(p, b + 1), length = p.lengths[b];
   r.rows = max(next - r.first, 0), r.length = max(length, 0);
   r.tokens = min(r.length, p.places);
-  r.begin = p.window ? behind(r.length - r.rows + 1, p.window) & ~15 : 0;
+  r.begin = p.window ? min(behind(r.length - r.rows + 1, p.window), r.tokens) & ~15 : 0;  // (at most places: what is added to it stays in 32 bits)
   r.blocks = (max(r.tokens - r.begin, 0) + BLOCK - 1) / BLOCK;
   r.tiles = (r.rows * p.group + (1 << p.plan.tile_log) - 1) >> p.plan.tile_log;
   return r;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
     seen_from = p.window ? behind(sees + bottom, p.window) : 0;
     seen_to = min(sees + top, r.tokens);
     last = top < r.rows ? min(sees + bottom, r.tokens) : 0;
-    window_begin = p.window ? behind(sees + top, p.window) & ~15 : 0;
+    window_begin = p.window ? min(behind(sees + top, p.window), r.tokens) & ~15 : 0;
   }
   const int slice_begin = r.begin + r.slice * r.size, end = __builtin_amdgcn_readfirstlane(min(slice_begin + r.size, last)), begin = max(slice_begin, window_begin);
   seen_from = __builtin_amdgcn_readfirstlane(seen_from), seen_to = __builtin_amdgcn_readfirstlane(min(seen_to, end));
