@@ -111,6 +111,7 @@ REFUSALS = [
     ("tts_qk_norm_rope", rope_args, dict(w_k=tensor(F32, 64, ptr=FAR[5])), N.TTS_INVALID, "w_k is f32, not bf16"),
     ("tts_qk_norm_rope", rope_args, dict(eps=-1.0), N.TTS_INVALID, "eps"),
     ("tts_qk_norm_rope", rope_args, dict(eps=NAN), N.TTS_INVALID, "eps"),
+    ("tts_qk_norm_rope", rope_args, dict(eps=1e39), N.TTS_INVALID, "eps"),
     ("tts_qk_norm_rope", rope_args, dict(q_out=tensor(BF16, 5, 8, 64, stride=(512, 32, 1), ptr=FAR[6])), N.TTS_INVALID, "q_out: its rows overlap"),
     ("tts_qk_norm_rope", rope_args, dict(q_out=tensor(BF16, 5, 8, 64, ptr=FAR[0] + 2)), N.TTS_INVALID, "q_out shares memory with q"),
     ("tts_qk_norm_rope", rope_args, dict(k_out=tensor(BF16, 5, 2, 64, ptr=FAR[0])), N.TTS_INVALID, "k_out shares memory with q"),
@@ -140,11 +141,14 @@ REFUSALS = [
     ("tts_kv4_attention", attend_args, dict(window=-1), N.TTS_INVALID, "window is -1"),
     ("tts_kv4_attention", attend_args, dict(longest=-1), N.TTS_INVALID, "longest is -1"),
     ("tts_kv4_attention", attend_args, dict(scale=INF), N.TTS_INVALID, "scale"),
+    ("tts_kv4_attention", attend_args, dict(scale=-1e39), N.TTS_INVALID, "scale"),
     ("tts_kv4_attention", attend_args, dict(out=tensor(BF16, 5, 8, 64, ptr=FAR[1] + 2)), N.TTS_INVALID, "out shares memory with q"),
     ("tts_kv4_attention", attend_args, dict(out=tensor(BF16, 5, 8, 64, ptr=FAR[0] + 128)), N.TTS_INVALID, "out shares memory with cache"),
     ("tts_kv4_attention", attend_args, dict(table=tensor(I32, 3, 1000, ptr=FAR[2]), bytes=16), N.TTS_INVALID, "the workspace has 16 bytes"),
     ("tts_kv4_attention", attend_args, dict(table=tensor(I32, 3, 1000, ptr=FAR[2]), work=None), N.TTS_INVALID, "workspace is a null pointer"),
     ("tts_kv4_attention", attend_args, dict(q=tensor(BF16, 1 << 24, 8, 64, ptr=FAR[1])), N.TTS_UNSUPPORTED, "16777216 rows of 8 heads"),
+    ("tts_kv4_attention", attend_args, dict(q=tensor(BF16, 4097, 4095, 32, ptr=FAR[1]), cache=cache_t(heads=4095, dim=32), table=tensor(I32, 4097, 4, ptr=FAR[2]), lengths=tensor(I32, 4097, ptr=FAR[3]),
+                                            starts=tensor(I32, 4098, ptr=FAR[4]), out=tensor(BF16, 4097, 4095, 32, ptr=FAR[5])), N.TTS_UNSUPPORTED, "4097 requests of 4095 heads"),   # 2^24 - 1 workgroups and 8
 ]
 
 

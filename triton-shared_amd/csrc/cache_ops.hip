@@ -69,8 +69,8 @@ struct Attend {
     p.places = (int)most;
     p.by_group = fast_div(p.group), p.by_heads = fast_div(p.heads);
     p.plan = plan_attend(p.tokens, p.requests, p.heads, p.cache.heads, p.cache.dim, longest ? std::min(longest, most) : most, window);
-    // (a launch of 2^32 lanes and more starts only their remainder)
-    if ((p.plan.items + p.plan.extra) * p.cache.heads >= (1 << 24)) unsupported(std::to_string(p.requests) + " requests of " + std::to_string(p.cache.heads) + " heads: more workgroups than a launch has");
+    // (a launch of 2^32 lanes and more starts only their remainder; the rows of no request have 8 workgroups besides)
+    if ((p.plan.items + p.plan.extra) * p.cache.heads + 8 >= (1 << 24)) unsupported(std::to_string(p.requests) + " requests of " + std::to_string(p.cache.heads) + " heads: more workgroups than a launch has");
   }
 };
 
@@ -130,7 +130,7 @@ tts_status tts_qk_norm_rope(const tts_tensor *q_, const tts_tensor *k_, const tt
     cos_sin.rank(2).type(TTS_F32).neighbours();
     const int64_t rotary = cos_sin.size(1);
     if (rotary < 2 || rotary % 2 || rotary > dim) invalid("cos_sin: dimension 1 is " + std::to_string(rotary) + ", not an even number up to q's " + std::to_string(dim));
-    if (!(eps >= 0.0) || !std::isfinite(eps)) invalid("eps is " + std::to_string(eps));
+    if (!(eps >= 0.0) || !std::isfinite((float)eps)) invalid("eps is " + std::to_string(eps));
     RopeParams p = {};
     p.w_f32 = 0;
     if (!w_q_ != !w_k_) invalid(std::string(w_q_ ? "w_k" : "w_q") + " is missing");
@@ -195,7 +195,7 @@ tts_status tts_kv4_attention(const tts_tensor *q_, const tts_tensor *cache_, con
     lengths.rank(1).type(TTS_I32).shape(0, p.requests, "table").neighbours();
     starts.rank(1).type(TTS_I32).shape(0, (int64_t)p.requests + 1, "table").neighbours();
     out.rank(3).type(a.q.t->dtype).shape(0, p.tokens, "q").shape(1, p.heads, "q").shape(2, p.cache.dim, "q").neighbours().distinct();
-    if (!std::isfinite(scale)) invalid("the scale is " + std::to_string(scale));
+    if (!std::isfinite((float)scale)) invalid("the scale is " + std::to_string(scale));
     for (const Arg *x : {&a.q, &a.table, &lengths, &starts, &out}) x->present();
     same_or_apart(out, a.q);
     apart(out, a.cache), apart(out, a.table), apart(out, lengths), apart(out, starts);
