@@ -190,6 +190,13 @@ def test_workspaces_hold_the_slices():
     assert N.lib().tts_kv4_attention_workspace(q, cache, tensor(I32, 4, 1000, ptr=FAR[2]), 0, 1 << 40, ctypes.byref(size)) == 0 and size.value == long
 
 
+def test_strides_of_single_pages_and_heads_say_nothing():
+    L, size = N.lib(), ctypes.c_size_t()
+    for heads, pages, stride, status in ((1, 10, (576, 1, 1), 0), (2, 1, (1, 576, 1), 0), (1, 1, (5, 3, 1), 0), (2, 10, (1152, 577, 1), N.TTS_INVALID), (1, 10, (577, 1, 1), N.TTS_INVALID)):
+        cache = tensor(BF16, pages, heads, 576, stride=stride)
+        assert L.tts_kv4_attention_workspace(tensor(BF16, 4, 8, 64, ptr=FAR[1]), cache, tensor(I32, 4, 4, ptr=FAR[2]), 0, 0, ctypes.byref(size)) == status
+
+
 def test_python_arguments_are_checked_without_a_gpu():
     cpu = torch.zeros(4, 16, dtype=torch.int32)
     with pytest.raises(TypeError, match="GPU memory"):

@@ -23,7 +23,7 @@ Kv4Cache cache_of(const Arg &a, int64_t dim) {
   if (a.size(0) < 1 || a.size(1) < 1) invalid(a.name + " is empty");
   if (a.size(0) * page > INT_MAX) unsupported(a.name + ": " + std::to_string(a.size(0) * page) + " slots, more than 32 bits number");
   if (a.size(1) > 65535) unsupported(a.name + ": " + std::to_string(a.size(1)) + " heads");
-  if (a.first() % 16 || a.stride(0) % 8 || a.stride(1) % 8) invalid(a.name + ": its pages and heads do not begin at multiples of 16 bytes");
+  if (a.first() % 16 || (a.size(0) > 1 && a.stride(0) % 8) || (a.size(1) > 1 && a.stride(1) % 8)) invalid(a.name + ": its pages and heads do not begin at multiples of 16 bytes");
   a.present();
   Kv4Cache c = {};
   c.base = a.t->ptr, c.page_bytes = a.stride(0) * 2, c.head_bytes = a.stride(1) * 2;
