@@ -1076,3 +1076,49 @@ def test_results_do_not_change_from_call_to_call():
         first = call()
         for _ in range(5):
             assert torch.equal(call(), first)
+
+
+# A step with more new tokens than rows: those that have one are where `page_slots` says, and see nothing behind themselves (never written, the others are NaN here)
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,fresh,rows,Hq,Hk,longest", [
+    ([5], [5], 3, 4, 2, None), ([40, 90, 33], [1, 7, 2], 4, 8, 2, None), ([40, 90, 33], [1, 7, 2], 8, 8, 2, None),
+    ([9000, 30], [40, 1], 17, 8, 2, None),                                                           # in slices
+    ([70, 300, 1, 129], [3, 5, 1, 4], 7, 64, 64, 100),                                               # wavefronts with heads of their own
+    ([250, 391, 171], [240, 391, 150], 500, 64, 64, None), ([250, 391], [240, 391], 301, 192, 32, None),  # ... with rows of their own
+])
+def test_attend_of_fewer_rows_than_new_tokens(lengths, fresh, rows, Hq, Hk, longest):
+    a = make_attend(lengths, fresh, Hq, Hk, 64, seed=rows)
+    table = a["table"].clone()
+    taken = [a["table"][b, c].item() for b, (n, f) in enumerate(zip(lengths, fresh)) for c in range(-(-(n - f) // 16), -(-n // 16))]
+    slots, positions, _, starts, _ = ops.page_slots(table, a["lengths"], ints(fresh), ints(taken[::-1]), ints([len(taken)]), 16, rows)
+    assert torch.equal(table, a["table"]) and torch.equal(starts, a["starts"])
+    at, want_at = starts.tolist(), []
+    for n, f, first in zip(lengths, fresh, at):
+        want_at += list(range(n - f, n))
+    assert positions.tolist() == want_at[:rows]
+    k, v = a["k"].clone(), a["v"].clone()
+    for b, (n, f) in enumerate(zip(lengths, fresh)):
+        for j in range(n - f + min(max(rows - at[b], 0), f), n):
+            k[int(table[b, j // 16]) * 16 + j % 16], v[int(table[b, j // 16]) * 16 + j % 16] = NAN, NAN
+    kept = fill(a | dict(k=k, v=v), 16)
+    assert bool((slots >= 0).all())
+    for window in (None, 1, 20):
+        want, lim, _ = attend_exact(a, 0.125, window)
+        got = ops.kv4_attention(a["q"][:rows], kept["cache"], table, a["lengths"], starts, window=window, longest=longest)
+        assert bool(((got.double() - want[:rows]).abs() <= lim[:rows]).all())
+
+
+@pytest.mark.gpu
+def test_steps_with_more_new_tokens_than_rows():
+    # all of a step's operators: the first rows of a step that has them all
+    fresh = [30, 1, 70]
+    whole, cut = Session(3, 40), Session(3, 40)
+    for n, rows in enumerate([101, 100, 60, 31, 30, 7]):
+        x = gpu(101, 12, 64, seed=n, dtype="bf16")
+        for s in (whole, cut):
+            s.table.fill_(-1), s.lengths.zero_(), s.count.fill_(40)
+        want, got = whole.step(x, ints(fresh)), cut.step(x[:rows], ints(fresh))
+        for a, b in zip(want[1:7], got[1:7]):
+            assert torch.equal(a[:rows], b)
+        # (each within half a step of bf16 and 2^-11 of the codes' part of what is exact, and that is less than 15 steps, some 6)
+        assert bool(((got[0].double() - want[0][:rows].double()).abs() <= 2.0 ** -6 * want[0][:rows].double().abs() + 0.02).all())

@@ -72,7 +72,7 @@ __device__ __forceinline__ u32 fp16_pair(float a, float b) {
 struct Work {
   int request, first, rows;     // of the step's rows: where the request's begin, and how many it has (0: nothing to do)
   int tile, slice, slices;
-  int length, tokens;           // of the request, and how many of them the table can hold
+  int length, tokens;           // up to the last of these rows, and how many of them the table can hold
   int begin, size;              // the first token that its rows see, at a multiple of 16, and a slice's tokens
   int index;                    // of its first workgroup
 };
@@ -91,8 +91,9 @@ __device__ __forceinline__ Request request_of(const AttendParams &p, int b) {
   if (b >= p.requests) return r;
   r.first = start_of(p, b);
   const int next = start_of(p, b + 1), length = p.lengths[b];
-  r.rows = max(next - r.first, 0), r.length = max(length, 0);
-  r.tokens = min(r.length, p.places);
+  // (of more new tokens than q has rows the first have one, and what lies behind them is none of theirs to see; far below 0 nothing changes any more)
+  r.rows = max(next - r.first, 0), r.length = max(max(length, 0) - (max(p.starts[b + 1], 0) - next), -(1 << 30));
+  r.tokens = min(max(r.length, 0), p.places);
   r.begin = p.window ? min(behind(r.length - r.rows + 1, p.window), r.tokens) & ~15 : 0;  // (at most places: what is added to it stays in 32 bits)
   r.blocks = (max(r.tokens - r.begin, 0) + BLOCK - 1) / BLOCK;
   r.tiles = (r.rows * p.group + (1 << p.plan.tile_log) - 1) >> p.plan.tile_log;
