@@ -1083,7 +1083,7 @@ def test_results_do_not_change_from_call_to_call():
 @pytest.mark.parametrize("lengths,fresh,rows,Hq,Hk,longest", [
     ([5], [5], 3, 4, 2, None), ([40, 90, 33], [1, 7, 2], 4, 8, 2, None), ([40, 90, 33], [1, 7, 2], 8, 8, 2, None),
     ([9000, 30], [40, 1], 17, 8, 2, None),                                                           # in slices
-    ([70, 300, 1, 129], [3, 5, 1, 4], 7, 64, 64, 100),                                               # wavefronts with heads of their own
+    ([70, 300, 1, 129], [3, 5, 1, 4], 7, 64, 64, 60),                                                # wavefronts with heads of their own
     ([250, 391, 171], [240, 391, 150], 500, 64, 64, None), ([250, 391], [240, 391], 301, 192, 32, None),  # ... with rows of their own
 ])
 def test_attend_of_fewer_rows_than_new_tokens(lengths, fresh, rows, Hq, Hk, longest):
@@ -1122,3 +1122,53 @@ def test_steps_with_more_new_tokens_than_rows():
             assert torch.equal(a[:rows], b)
         # (each within half a step of bf16 and 2^-11 of the codes' part of what is exact, and that is less than 15 steps, some 6)
         assert bool(((got[0].double() - want[0][:rows].double()).abs() <= 2.0 ** -6 * want[0][:rows].double().abs() + 0.02).all())
+
+
+# Calls of each kind: tiles of 4, of 8 and of 16 rows, slices, wavefronts with heads and with rows of their own
+KINDS = {"4": ([300, 1, 70], [1, 1, 1], 8, 2, None), "8": ([300, 1, 70], [1, 1, 1], 16, 2, None), "16": ([300, 40], [40, 40], 8, 2, None), "slices": ([6000, 1], [1, 1], 8, 2, None),
+         "heads": ([70, 300, 1, 0, 129, 64, 17, 1090], [1, 1, 1, 0, 3, 2, 1, 1], 64, 64, 100), "rows": ([250, 391, 171], [240, 391, 150], 64, 64, None)}
+
+
+# Scores past 2^24, the largest of 32 bits between which whole numbers lie: those that are the same count the same ...
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,size", [(128, 4000.0), (64, 8000.0), (32, 60000.0)])
+def test_attend_large_scores_that_are_the_same(D, size, dtype, kind):
+    lengths, fresh, Hq, Hk, longest = KINDS[kind]
+    a = make_attend(lengths, fresh, Hq, Hk, D, 16, dtype, seed=D)
+    sign = torch.where(torch.arange(len(a["q"]) * Hq, device="cuda") % 3 == 0, -1.0, 1.0).reshape(-1, Hq, 1)
+    a = fill(a | dict(k=torch.full_like(a["k"], size), q=(torch.full_like(a["q"], size) * sign).to(a["q"].dtype)), 16)
+    for window in (None, 30):
+        want, lim, _ = attend_exact(a, 0.0, window)  # (by the same scores without them)
+        got = ops.kv4_attention(a["q"], a["cache"], a["table"], a["lengths"], a["starts"], window=window, longest=longest)
+        assert bool(((got.double() - want).abs() <= lim).all())
+
+
+# ... and of others the largest alone: a key's elements are one number of -32 to 32 and three times that, and scores its products with 2^23 and more
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attend_large_scores_of_which_one_counts(sign, dtype, kind):
+    lengths, fresh, Hq, Hk, longest = KINDS[kind]
+    a = make_attend(lengths, fresh, Hq, Hk, 64, 16, dtype, seed=3)
+    level = (torch.arange(len(a["k"]), device="cuda") * 7 % 32 + 1).to(a["k"].dtype)
+    level[::2] *= -1
+    each = 1 + 2 * (torch.arange(64, device="cuda") % 2).to(level.dtype)  # (three times as much, within 2^-8 as it is held: no other order)
+    a = fill(a | dict(k=(level[:, None, None] * each).expand_as(a["k"]).contiguous(), q=torch.full_like(a["q"], 32768.0 * sign)), 16)
+    got = ops.kv4_attention(a["q"], a["cache"], a["table"], a["lengths"], a["starts"], scale=4.0, longest=longest)
+    assert bool(got.isfinite().all())
+    code, step, low = held(a["v"])
+    v, at = code * step + low, a["starts"].tolist()
+    for b, (n, f) in enumerate(zip(lengths, fresh)):
+        j = torch.arange(n, device="cuda")
+        slots = a["table"][b].long()[j // 16] * 16 + j % 16
+        z = level[slots].double() * sign
+        for r in range(f):
+            seen = slots[:n - f + r + 1]
+            chosen = seen[z[:n - f + r + 1] == z[:n - f + r + 1].max()]
+            want = v[chosen].mean(dim=0).repeat_interleave(Hq // Hk, dim=0)
+            # the values in 32 bits; weights that are the same, of which each may be off by 2^-11 of 15 steps; sums of as many; the rounding
+            lim = 2.0 ** -11 * 15 * step[chosen].amax() + 2.0 ** -16 * v[chosen].abs().amax() + half(dtype) * want.abs()
+            assert bool(((got[at[b] + r].double() - want).abs() <= lim).all())

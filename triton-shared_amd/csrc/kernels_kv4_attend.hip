@@ -380,8 +380,9 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
             const f32x4 step_v = *(const f32x4 *)(value_step + at + 16 * (2 * h + j)), low_v = *(const f32x4 *)(value_low + at + 16 * (2 * h + j));
             for (int i = 0; i < 4; i++) {
               const float score = s[2 * h + j][t][i];
-              const bool ok = !decltype(checked)::value || score != -__builtin_inff();
-              e[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score, factor[t], shift));
+              constexpr bool apart = decltype(checked)::value;
+              const bool ok = !apart || score != -__builtin_inff();
+              e[j][i] = __builtin_amdgcn_exp2f(apart ? (score - from) * factor[t] : __builtin_fmaf(score, factor[t], shift));
               st[j][i] = ok ? step_v[i] : 0.f;
               sum += e[j][i];
               base = __builtin_fmaf(e[j][i], ok ? low_v[i] : 0.f, base);
@@ -406,7 +407,8 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
             weights[t][part][1] = make_uint4(dpp_moved<0x108>(w.x), dpp_moved<0x108>(w.y), dpp_moved<0x108>(w.z), dpp_moved<0x108>(w.w));  // row_shl 8
           }
       };
-      if (careful) weigh(std::true_type{});
+      // (one rounding of the maximum instead of a difference per score: of up to 2^12 it is off by 2^-12, of 2^27 it would make weights of 16, or of 0)
+      if (careful || __any(!(fabsf(shift) <= 0x1p12f))) weigh(std::true_type{});
       else weigh(std::false_type{});
       total[t] += sum, lowest[t] += base;
     }
