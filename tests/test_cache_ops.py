@@ -1172,3 +1172,27 @@ def test_attend_large_scores_of_which_one_counts(sign, dtype, kind):
             # the values in 32 bits; weights that are the same, of which each may be off by 2^-11 of 15 steps; sums of as many; the rounding
             lim = 2.0 ** -11 * 15 * step[chosen].amax() + 2.0 ** -16 * v[chosen].abs().amax() + half(dtype) * want.abs()
             assert bool(((got[at[b] + r].double() - want).abs() <= lim).all())
+
+
+# Elements of q near the end of bf16, with keys that make ordinary scores of them; scales at both ends of 32 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("q_scale,k_scale,scale", [(1e36, 1e-36, None), (2.0 ** 124, 2.0 ** -124, None), (2.0 ** 100, 2.0 ** -100, 0.3), (1e-20, 1e-6, 1e26), (2.0 ** -100, 1.0, 2.0 ** 100), (1.0, 1e-30, 1e30), (1e30, 1e8, 1e-38),
+                                                   (1.0, 1e20, 1e-41), (1e-36, 1e36, None)])
+def test_attend_rows_and_scales_near_the_ends(q_scale, k_scale, scale, kind):
+    lengths, fresh, Hq, Hk, longest = KINDS[kind]
+    a = make_attend(lengths, fresh, Hq, Hk, 64, seed=5)
+    a = fill(a | dict(q=(a["q"].float().clamp(-5, 5) * q_scale).bfloat16(), k=(a["k"].float() * k_scale).bfloat16()), 16)
+    assert bool(a["q"].isfinite().all() and a["k"].isfinite().all())
+    check_attend(a, scale=scale, longest=longest)
+    # rows of all sizes side by side
+    mixed = a["q"].clone()
+    mixed[:, ::3] = (mixed[:, ::3].float() / q_scale).bfloat16()
+    check_attend(a | dict(q=mixed), scale=scale, longest=longest)
+
+
+@pytest.mark.gpu
+def test_attend_rows_whose_sum_is_not_finite():
+    a = make_attend([30, 70], [1, 40], 4, 2, 128, seed=5)
+    q = a["q"].abs().clamp(0.5, 1.0) * 2.0 ** 127  # 32 bits hold no sum of four
+    check_attend(fill(a | dict(q=q, k=a["k"] * 2.0 ** -120), 16))

@@ -166,7 +166,7 @@ constexpr int row_tiles_of(int w) { return w <= 4 ? 2 : 1; }
 // tiles of tokens, it goes on with 4 ROWS / 16 of them: the copies share the softmax.
 template <bool BF16, int W, int RT, int ROWS, int OWN>
 __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 && ROWS == 16) ? 2 : 3) void kv4_attend_kernel(AttendParams p) {
-  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK, WAVE_ROWS = RT * ROWS, TILE = (OWN == OWN_ROWS ? WAVES : 1) * WAVE_ROWS;
+  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_ROWS = RT * ROWS, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK + 4 * WAVE_ROWS, TILE = (OWN == OWN_ROWS ? WAVES : 1) * WAVE_ROWS;
   constexpr int BANKS = 16 / ROWS, NJ = 4 / BANKS;
   constexpr int MEET_PITCH = D + 4, MEET_BYTES = OWN != OWN_BLOCKS ? 0 : WAVES * WAVE_ROWS * (MEET_PITCH + 2) * 4;
   __shared__ __attribute__((aligned(16))) char lds[MEET_BYTES > WAVES * WAVE_BYTES ? MEET_BYTES : WAVES * WAVE_BYTES];
@@ -189,6 +189,7 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
 
   char *const mine = lds + wave * WAVE_BYTES;
   float *const key_step = (float *)(mine + V_BYTES), *const key_low = key_step + BLOCK, *const value_step = key_low + BLOCK, *const value_low = value_step + BLOCK;
+  float *const lifts = value_low + BLOCK;  // of the rows
   const int row0 = r.tile * TILE + (OWN == OWN_ROWS ? wave * WAVE_ROWS : 0);  // of the request's tokens and the group's heads
 
   // The rows, what they see, and q, on its way
@@ -268,27 +269,33 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
     load_keys();
   }
   // q as operands
-  float factor[RT], sum_q[RT];  // scores (in powers of two) are factor * (codes' product * step + lowest * sum_q)
+  // (A score in powers of two is factor * lift * (codes' product * step + lowest * sum of q): the lift is 1, but 2^40 where 32 bits cannot hold the factor without it, of rows with elements of 2^85 and
+  // more.  It holds wherever the scale times the row's largest element is finite in 32 bits.)
+  float factor[RT], sum_q[RT];
   uint4 q[RT][W];
+  bool lifted = false;
   for (int t = 0; t < RT; t++) {
     float v[W][8], most = 0.f, sum = 0.f;
     for (int w = 0; w < W; w++)
       for (int e = 0; e < 8; e++) {
         v[w][e] = half_of(raw[t][w].d[e / 2], BF16, e & 1);  // (of a row that is not there: the first's, for nothing)
-        most = fmaxf(most, fabsf(v[w][e])), sum += v[w][e];
+        most = fmaxf(most, fabsf(v[w][e]));
       }
     most = over_row(most, [](float a, float b) { return fmaxf(a, b); });
-    sum = over_row(sum, [](float a, float b) { return a + b; });
     const int power_q = most > 0.f && most < __builtin_inff() ? max(-126, min(126, 14 - __builtin_amdgcn_frexp_expf(most))) : 0;
     const float sign = __builtin_amdgcn_ldexpf(p.scale < 0.f ? -1.f : p.scale == 0.f ? 0.f : 1.f, power_q);
     for (int w = 0; w < W; w++) {
       float x[8];
-      for (int e = 0; e < 8; e++) x[e] = v[w][e] * (e & 2 ? sign * 0x1p-4f : sign);
+      for (int e = 0; e < 8; e++) x[e] = v[w][e] * (e & 2 ? sign * 0x1p-4f : sign), sum += v[w][e] * sign;
       q[t][w] = make_uint4(fp16_pair(x[0], x[1]), fp16_pair(x[2], x[3]), fp16_pair(x[4], x[5]), fp16_pair(x[6], x[7]));
     }
-    factor[t] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(p.scale) * LOG2_E, 24 - power_q), 0x1p-126f);
+    sum = over_row(sum, [](float a, float b) { return a + b; });
+    const bool far = !(__builtin_amdgcn_ldexpf(fabsf(p.scale), 24 - power_q) < 0x1p100f);
+    factor[t] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(p.scale), (far ? -16 : 24) - power_q) * LOG2_E, 0x1p-149f);
     // (a row with an infinity: NaN, as the formula gives, also where all its scores are -inf here)
-    sum_q[t] = (sum - sum == 0.f ? sum : __builtin_nanf("")) * sign * 0x1p-24f;
+    sum_q[t] = (sum - sum == 0.f ? sum : __builtin_nanf("")) * (far ? 0x1p16f : 0x1p-24f);
+    lifts[t * ROWS + m % ROWS] = far ? 0x1p40f : 1.f;
+    lifted = lifted || __any(far);
   }
   f32x4 out[D / 16][RT];
   float top[RT], total[RT], lowest[RT];
@@ -336,6 +343,12 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
           for (int t = 0; t < RT; t++) all[j][t] = mfma16<false>(k, q[t][w], all[j][t]);
         }
       }
+      if (lifted)
+        for (int t = 0; t < RT; t++) {
+          const float lift = lifts[t * ROWS + m % ROWS];
+          for (int j = 0; j < 4; j++)
+            for (int i = 0; i < 4; i++) all[j][t][i] *= lift;
+        }
       for (int t = 0; t < RT; t++)
         for (int j = 0; j < NJ; j++)
           for (int i = 0; i < 4; i++) {
