@@ -191,7 +191,8 @@ tts_status tts_kv4_write(const tts_tensor *cache, const tts_tensor *k, const tts
 tts_status tts_kv4_read(const tts_tensor *cache, const tts_tensor *slots, const tts_tensor *k, const tts_tensor *v, void *stream);
 
 /* Attention over the cache.  q [T, Hq, D], out the same (it may be q), Hq a multiple of Hk: head h reads the cache's head h / (Hq / Hk).  Rows starts[b] .. starts[b + 1] - 1 of q
- * are the last tokens of request b, which has lengths[b] tokens in the cache, in the pages table[b] (M columns; starts [B + 1], lengths [B], table [B, M] i32); the one at
+ * are the last tokens of request b, which has lengths[b] tokens in the cache, in the pages table[b] (M columns, places for less than 2^30 tokens; starts [B + 1], lengths [B], table
+ * [B, M] i32); the one at
  * position i sees tokens j <= i, with a window (not 0) i - window < j, whose page is in the table and in [0, pages).  Where starts[B] is past T, the rows that there are have the positions
  * that page_slots gives them.
  *   out = sum over j of e^(z_j) v_j / sum of e^(z_j),  z_j = scale * q . k_j;  zeros for a row that sees none; rows of no request (before starts[0], behind starts[B])

@@ -1196,3 +1196,13 @@ def test_attend_rows_whose_sum_is_not_finite():
     a = make_attend([30, 70], [1, 40], 4, 2, 128, seed=5)
     q = a["q"].abs().clamp(0.5, 1.0) * 2.0 ** 127  # 32 bits hold no sum of four
     check_attend(fill(a | dict(q=q, k=a["k"] * 2.0 ** -120), 16))
+
+
+# (no GPU needed: tokens that a row of the table has places for and that the kernel would leave out)
+@pytest.mark.parametrize("columns,page,longest,refused", [((1 << 26) - 1, 16, 0, False), (1 << 26, 16, 0, True), (1 << 26, 16, 1000, True), ((1 << 14) - 1, 1 << 16, 0, False), (1 << 14, 1 << 16, 0, True), (1 << 30, 16, 0, True)])
+def test_tables_with_places_for_2_30_tokens_are_refused(columns, page, longest, refused):
+    bytes_ = ctypes.c_size_t()
+    status = N.lib().tts_kv4_attention_workspace(tensor(BF16, 1, 8, 32, ptr=FAR[1]), cache_t(pages=10, page=page, dim=32), tensor(I32, 1, columns, ptr=FAR[2]), 0, longest, ctypes.byref(bytes_))
+    assert status == (N.TTS_UNSUPPORTED if refused else N.TTS_OK)
+    if refused:
+        assert f"places for {columns * page} tokens" in N.lib().tts_last_error().decode()

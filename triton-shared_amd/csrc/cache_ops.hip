@@ -65,7 +65,8 @@ struct Attend {
     if (longest < 0) invalid("longest is " + std::to_string(longest));
     if (p.tokens * p.heads > ((int64_t)1 << 26)) unsupported("q: " + std::to_string(p.tokens) + " rows of " + std::to_string(p.heads) + " heads");
     if (p.requests > (1 << 20)) unsupported("table: " + std::to_string(p.requests) + " requests");
-    const int64_t most = std::min(table.size(1) * p.cache.page, (int64_t)INT_MAX / 2);
+    const int64_t most = table.size(1) * p.cache.page;
+    if (most > INT_MAX / 2) unsupported("table: places for " + std::to_string(most) + " tokens, 2^30 and more");  // (what is added to a token's number stays in 32 bits)
     p.places = (int)most;
     p.by_group = fast_div(p.group), p.by_heads = fast_div(p.heads);
     p.plan = plan_attend(p.tokens, p.requests, p.heads, p.cache.heads, p.cache.dim, longest ? std::min(longest, most) : most, window);

@@ -304,7 +304,7 @@ def kv4_attention(q, cache, table, lengths, starts, scale=None, window=None, lon
     q [T, Hq, D] of the cache's type, Hq a multiple of its heads: head h reads the cache's head h // (Hq // Hk).  Rows starts[b] .. starts[b + 1] - 1 are the last tokens of request b, which has
     lengths[b] tokens in the pages table[b] (table [B, M], lengths [B], starts [B + 1], all int32, as `page_slots` leaves them); the row at position i sees the tokens j <= i, with a
     `window` those of i - window < j.  scale is D ** -0.5 unless it is given.  A row that sees nothing is zeros; rows of no request are zeros too, or as they were in an `out` that is given (it may be q).
-    `longest`, a length that no request passes, lets short requests in a wide table do with fewer workgroups.
+    `longest`, a length that no request passes, lets short requests in a wide table do with fewer workgroups.  A table's row has places for less than 2^30 tokens.
     """
     if window is not None and _whole("window", window) < 1:
         raise ValueError(f"window is {window}")
