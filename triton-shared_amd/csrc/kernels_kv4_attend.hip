@@ -343,12 +343,6 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
           for (int t = 0; t < RT; t++) all[j][t] = mfma16<false>(k, q[t][w], all[j][t]);
         }
       }
-      if (lifted)
-        for (int t = 0; t < RT; t++) {
-          const float lift = lifts[t * ROWS + m % ROWS];
-          for (int j = 0; j < 4; j++)
-            for (int i = 0; i < 4; i++) all[j][t][i] *= lift;
-        }
       for (int t = 0; t < RT; t++)
         for (int j = 0; j < NJ; j++)
           for (int i = 0; i < 4; i++) {
@@ -357,6 +351,12 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
           }
     }
     if (n + 1 < blocks) load_keys();
+    if (lifted)
+      for (int t = 0; t < RT; t++) {
+        const float lift = lifts[t * ROWS + m % ROWS];
+        for (int j = 0; j < NJ; j++)
+          for (int i = 0; i < 4; i++) s[j][t][i] *= lift;
+      }
     const int at = 16 * NJ * bank + 4 * g;  // the first of a lane's tokens in the block
     for (int j = 0; j < NJ; j++) {
       const f32x4 step_k = *(const f32x4 *)(key_step + at + 16 * j), low_k = *(const f32x4 *)(key_low + at + 16 * j);
