@@ -1206,3 +1206,35 @@ def test_tables_with_places_for_2_30_tokens_are_refused(columns, page, longest, 
     assert status == (N.TTS_UNSUPPORTED if refused else N.TTS_OK)
     if refused:
         assert f"places for {columns * page} tokens" in N.lib().tts_last_error().decode()
+
+
+# Values of a token that most rows do not see, far larger than theirs, or none: rows that do not see it are what they are without it, bit by bit
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,fresh,Hq,Hk,longest", [([300, 40], [40, 40], 8, 2, None), ([9, 130], [5, 3], 8, 2, None), ([200, 70], [3, 2], 6, 3, None), ([6000, 2000], [3, 3], 16, 2, None), ([3500, 90], [200, 90], 2, 1, None),
+                                                         ([70, 300, 1, 0, 129, 64, 17, 1090], [1, 1, 1, 0, 3, 2, 1, 3], 64, 64, 100), ([250, 391, 171], [240, 391, 150], 64, 64, None), ([260, 401], [220, 130], 192, 32, None)])
+@pytest.mark.parametrize("dtype,window", [("bf16", None), ("bf16", 2), ("bf16", 70), ("fp16", None), ("fp16", 70)])
+def test_attend_of_large_values_that_rows_do_not_see(lengths, fresh, Hq, Hk, longest, dtype, window):
+    a = make_attend(lengths, fresh, Hq, Hk, 64, 16, dtype, seed=sum(lengths))
+    if dtype == "fp16":
+        a = fill(a | dict(v=a["v"] * 2.0 ** -12), 16)
+    plain = check_attend(a, window=window, longest=longest)
+    starts = a["starts"].tolist()
+    for size, back in [(1e10, 1), (1e10, 2), (2.0 ** 24, 65), (2.0 ** 120, 1), (NAN, 1), (INF, 65)]:  # the last token, or one that some rows no longer see
+        if dtype == "fp16":
+            size = min(size, 2.0 ** 24)
+        v, sees = a["v"].clone(), torch.zeros(len(a["q"]), dtype=torch.bool, device="cuda")
+        for b, (n, f) in enumerate(zip(lengths, fresh)):
+            j = n - back
+            if j < 0:
+                continue
+            slot = int(a["table"][b, j // 16]) * 16 + j % 16
+            v[slot] = (v[slot].float() * size).to(v.dtype)
+            i = torch.arange(n - f, n, device="cuda")
+            sees[starts[b]:starts[b + 1]] = (i >= j) & ((i - j < window) if window else True)
+        x = fill(a | dict(v=v), 16)
+        if size == 1e10 or (dtype == "fp16" and back == 2):
+            got = check_attend(x, window=window, longest=longest)
+        else:
+            got = ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"], window=window, longest=longest)
+        assert torch.equal(got[~sees].view(torch.int16), plain[~sees].view(torch.int16))
+        assert size == size or bool(got[sees].isnan().all())

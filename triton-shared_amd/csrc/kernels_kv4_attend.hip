@@ -5,7 +5,7 @@
 // so the matrix instructions multiply codes.  A code in bits 0 .. 3 or 4 .. 7 of a half is the fp16 c 2^-24 or c 2^-20 (a number below the normal
 // ones, which they take as it is): eight codes of a 32-bit word become four pairs with four ands and one shift, and what is multiplied with the second kind is
 // 2^-4 of itself.  q goes in as fp16 times a power of two per row that takes its largest element to [2^13, 2^14): exactly, but for 2^-34 of that element.
-// p_j a'_j goes in as fp16, times a power of two per wavefront that takes the largest a' so far to [2^13, 2^14) and 2^-4 for every second token: within 2^-11 of it, less than the rounding of a
+// p_j a'_j goes in as fp16, times a power of two per row that takes the largest a' that it has seen so far to [2^13, 2^14) and 2^-4 for every second token: within 2^-11 of it, less than the rounding of a
 // bf16 output (2^-8); where the output is fp16 too, as the sum of two (2^-22); and within 2^-34 of the largest a'.  All sums and the statistics are in 32 bits.
 //
 // A wavefront takes blocks of 64 tokens.  Keys: lane (m, g) = (lane % 16, lane / 16) loads a quarter g of token m of each of four tiles, which is the
@@ -166,7 +166,7 @@ constexpr int row_tiles_of(int w) { return w <= 4 ? 2 : 1; }
 // tiles of tokens, it goes on with 4 ROWS / 16 of them: the copies share the softmax.
 template <bool BF16, int W, int RT, int ROWS, int OWN>
 __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 && ROWS == 16) ? 2 : 3) void kv4_attend_kernel(AttendParams p) {
-  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_ROWS = RT * ROWS, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK + 4 * WAVE_ROWS, TILE = (OWN == OWN_ROWS ? WAVES : 1) * WAVE_ROWS;
+  constexpr int D = 32 * W, PITCH = D / 2 + 8, V_BYTES = BLOCK * PITCH, WAVE_ROWS = RT * ROWS, WAVE_BYTES = V_BYTES + 4 * 4 * BLOCK + 4 * 2 * WAVE_ROWS, TILE = (OWN == OWN_ROWS ? WAVES : 1) * WAVE_ROWS;
   constexpr int BANKS = 16 / ROWS, NJ = 4 / BANKS;
   constexpr int MEET_PITCH = D + 4, MEET_BYTES = OWN != OWN_BLOCKS ? 0 : WAVES * WAVE_ROWS * (MEET_PITCH + 2) * 4;
   __shared__ __attribute__((aligned(16))) char lds[MEET_BYTES > WAVES * WAVE_BYTES ? MEET_BYTES : WAVES * WAVE_BYTES];
@@ -189,7 +189,8 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
 
   char *const mine = lds + wave * WAVE_BYTES;
   float *const key_step = (float *)(mine + V_BYTES), *const key_low = key_step + BLOCK, *const value_step = key_low + BLOCK, *const value_low = value_step + BLOCK;
-  float *const lifts = value_low + BLOCK;  // of the rows
+  float *const lifts = value_low + BLOCK;            // of the rows
+  int *const powers = (int *)(lifts + WAVE_ROWS);  // ... values' steps that it has seen are up to 2^power
   const int row0 = r.tile * TILE + (OWN == OWN_ROWS ? wave * WAVE_ROWS : 0);  // of the request's tokens and the group's heads
 
   // The rows, what they see, and q, on its way
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
     factor[t] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(p.scale), (far ? -16 : 24) - power_q) * LOG2_E, 0x1p-149f);
     // (a row with an infinity: NaN, as the formula gives, also where all its scores are -inf here)
     sum_q[t] = (sum - sum == 0.f ? sum : __builtin_nanf("")) * (far ? 0x1p16f : 0x1p-24f);
-    lifts[t * ROWS + m % ROWS] = far ? 0x1p40f : 1.f;
+    lifts[t * ROWS + m % ROWS] = far ? 0x1p40f : 1.f, powers[t * ROWS + m % ROWS] = -112;
     lifted = lifted || __any(far);
   }
   f32x4 out[D / 16][RT];
@@ -303,29 +304,60 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
     top[t] = -__builtin_inff(), total[t] = 0.f, lowest[t] = 0.f;
     for (int d = 0; d < D / 16; d++) out[d][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  int power = -112;  // values' steps so far are up to 2^power
-  float unit = __builtin_amdgcn_ldexpf(1.f, 14 - power), limit = __builtin_amdgcn_ldexpf(1.f, power);
+  // The rows' powers are the same as a rule, and value_step holds steps in their unit.  Where they are not (some have seen a larger step than others), or where rows must not see one that is past their
+  // power, it holds steps as they are, for each row to take in its own unit.
+  bool mixed = false;
+  float unit = 0x1p126f, limit = 0x1p-112f;  // of the least power; 2^ it
+  bool far[RT] = {};                         // exponents of some row are of the difference to its maximum
 
   for (int n = 0; n < blocks; n++) {
     const u32 present = (u32)(there >> (n % 16 * 4)) & 15;  // tiles
     // values and pairs to LDS: the 16 tokens of a lane's operand in a row, 8 bytes between rows
     for (int j = 0; j < 4; j++) __builtin_memcpy(mine + (m / 4 * 16 + j * 4 + m % 4) * PITCH + g * (4 * W), &values[j], 4 * W);
     const float step = half_of(value_pair, BF16, false), lowest_value = half_of(value_pair, BF16, true);
-    if (__any(step > limit && step < __builtin_inff())) {  // the largest so far: what there is in its unit
-      const float most = over_lanes<64>(step < __builtin_inff() ? step : 0.f, [](float a, float b) { return fmaxf(a, b); });
-      const int now = __builtin_amdgcn_frexp_expf(most);
-      const float moved = __builtin_amdgcn_ldexpf(1.f, max(power - now, -126));
-      for (int t = 0; t < RT; t++)
-        for (int d = 0; d < D / 16; d++)
-          for (int i = 0; i < 4; i++) out[d][t][i] *= moved;
-      power = now, unit = __builtin_amdgcn_ldexpf(1.f, 14 - power), limit = __builtin_amdgcn_ldexpf(1.f, power);
-    }
-    key_step[lane] = half_of(key_pair, BF16, false), key_low[lane] = half_of(key_pair, BF16, true);
-    value_step[lane] = step * (lane & 1 ? unit * 0x1p-4f : unit), value_low[lane] = lowest_value;
     const int first = start + n * STEP;
     const bool whole = first >= seen_from && first + BLOCK <= seen_to && present == 15;
+    const bool raises = step >= limit && step < __builtin_inff();
+    if (__builtin_expect(__any(raises), 0)) {  // the largest so far, for some row: what there is in its unit
+      const bool here = present >> g & 1, by_all = here && first + lane >= seen_from && first + lane < seen_to;
+      const float largest = over_lanes<64>(raises && by_all ? step : 0.f, [](float a, float b) { return fmaxf(a, b); });
+      const float reach = largest > 0.f ? __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(largest)) : 0.f;
+      float most[RT];
+      for (int t = 0; t < RT; t++) most[t] = largest;
+      if (__any(raises && !by_all && step >= reach)) {  // (of the others none matters beside what all rows see)
+        value_step[lane] = raises && here ? step : 0.f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        for (int t = 0; t < RT; t++) {
+          const int from = low[t] - first - 16 * g, to = min(high[t], end) - first - 16 * g;
+          float seen = 0.f;
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4 steps = *(const f32x4 *)(value_step + 16 * g + i);
+            for (int e = 0; e < 4; e++) seen = fmaxf(seen, i + e >= from && i + e < to ? steps[e] : 0.f);
+          }
+          most[t] = over_row(seen, [](float a, float b) { return fmaxf(a, b); });
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+      int least = 1024, greatest = -1024;
+      for (int t = 0; t < RT; t++) {
+        const int was = powers[t * ROWS + m % ROWS], now = most[t] > 0.f ? max(was, __builtin_amdgcn_frexp_expf(most[t])) : was;
+        const float moved = __builtin_amdgcn_ldexpf(1.f, max(was - now, -126));
+        for (int d = 0; d < D / 16; d++)
+          for (int i = 0; i < 4; i++) out[d][t][i] *= moved;
+        powers[t * ROWS + m % ROWS] = now;
+        if (high[t] > 0) least = min(least, now), greatest = max(greatest, now);  // (not of rows that are not there)
+      }
+      least = over_lanes<16>(least, [](int a, int b) { return min(a, b); }), greatest = over_lanes<16>(greatest, [](int a, int b) { return max(a, b); });
+      least = __builtin_amdgcn_readfirstlane(least), mixed = __builtin_amdgcn_readfirstlane(greatest) != least;
+      unit = __builtin_amdgcn_ldexpf(1.f, 14 - least), limit = __builtin_amdgcn_ldexpf(1.f, least);
+    }
     // a step or lowest value of NaN stays with the rows that see it: 0 times it is not 0
-    const bool careful = !whole && __any(!(fabsf(step) + fabsf(lowest_value) < __builtin_inff()));
+    const bool careful = mixed || (!whole && __any(!(fabsf(step) + fabsf(lowest_value) < __builtin_inff()) || step >= limit));
+    const float steps_unit = careful ? 1.f : unit;
+    key_step[lane] = half_of(key_pair, BF16, false), key_low[lane] = half_of(key_pair, BF16, true);
+    value_step[lane] = step * (lane & 1 ? steps_unit * 0x1p-4f : steps_unit), value_low[lane] = lowest_value;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (n + 1 < blocks) {
@@ -351,7 +383,7 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
           }
     }
     if (n + 1 < blocks) load_keys();
-    if (lifted)
+    if (__builtin_expect(lifted, 0))
       for (int t = 0; t < RT; t++) {
         const float lift = lifts[t * ROWS + m % ROWS];
         for (int j = 0; j < NJ; j++)
@@ -382,10 +414,15 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
         for (int d = 0; d < D / 16; d++)
           for (int i = 0; i < 4; i++) out[d][t][i] *= kept;
         top[t] = most;
+        // (one rounding of the maximum instead of a difference per score: of up to 2^12 it is off by 2^-12, of 2^27 it would make weights of 16, or of 0)
+        far[t] = __any(!(fabsf(shift) <= 0x1p12f));
       }
       float sum = 0.f, base = 0.f;
       auto weigh = [&](auto checked) __attribute__((always_inline)) {
         constexpr int J = NJ < 2 ? 1 : 2;  // tiles of a pair that are the lane's own
+        constexpr bool apart = decltype(checked)::value;
+        const bool by_difference = !(fabsf(shift) <= 0x1p12f);
+        const float own = apart && careful ? __builtin_amdgcn_ldexpf(1.f, 14 - powers[t * ROWS + m % ROWS]) : 1.f;
         // pairs of tiles 0 and 1, and of 2 and 3, into the lanes of bank 0 (the others' columns of `out` hold nothing of use)
         for (int h = 0; h < NJ / J; h++) {
           float e[2][4], st[2][4];
@@ -393,10 +430,9 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
             const f32x4 step_v = *(const f32x4 *)(value_step + at + 16 * (2 * h + j)), low_v = *(const f32x4 *)(value_low + at + 16 * (2 * h + j));
             for (int i = 0; i < 4; i++) {
               const float score = s[2 * h + j][t][i];
-              constexpr bool apart = decltype(checked)::value;
               const bool ok = !apart || score != -__builtin_inff();
-              e[j][i] = __builtin_amdgcn_exp2f(apart ? (score - from) * factor[t] : __builtin_fmaf(score, factor[t], shift));
-              st[j][i] = ok ? step_v[i] : 0.f;
+              e[j][i] = __builtin_amdgcn_exp2f(apart && by_difference ? (score - from) * factor[t] : __builtin_fmaf(score, factor[t], shift));
+              st[j][i] = !apart ? step_v[i] : ok ? step_v[i] * own : 0.f;
               sum += e[j][i];
               base = __builtin_fmaf(e[j][i], ok ? low_v[i] : 0.f, base);
             }
@@ -420,8 +456,7 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
             weights[t][part][1] = make_uint4(dpp_moved<0x108>(w.x), dpp_moved<0x108>(w.y), dpp_moved<0x108>(w.z), dpp_moved<0x108>(w.w));  // row_shl 8
           }
       };
-      // (one rounding of the maximum instead of a difference per score: of up to 2^12 it is off by 2^-12, of 2^27 it would make weights of 16, or of 0)
-      if (careful || __any(!(fabsf(shift) <= 0x1p12f))) weigh(std::true_type{});
+      if (__builtin_expect(careful || far[t], 0)) weigh(std::true_type{});
       else weigh(std::false_type{});
       total[t] += sum, lowest[t] += base;
     }
@@ -440,6 +475,7 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
   for (int t = 0; t < RT; t++) {
     const auto add = [](float a, float b) { return a + b; };
     total[t] = over_row<ROWS>(total[t], add), lowest[t] = over_row<ROWS>(lowest[t], add), top[t] *= factor[t];
+    const int power = powers[t * ROWS + m % ROWS];
     for (int d = 0; d < D / 16; d++)
       for (int i = 0; i < 4; i++) out[d][t][i] = __builtin_amdgcn_ldexpf(out[d][t][i], 10 + power) + lowest[t];
   }
