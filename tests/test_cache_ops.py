@@ -1238,3 +1238,38 @@ def test_attend_of_large_values_that_rows_do_not_see(lengths, fresh, Hq, Hk, lon
             got = ops.kv4_attention(x["q"], x["cache"], x["table"], x["lengths"], x["starts"], window=window, longest=longest)
         assert torch.equal(got[~sees].view(torch.int16), plain[~sees].view(torch.int16))
         assert size == size or bool(got[sees].isnan().all())
+
+
+def codes_part(a, scale, window):
+    """What the codes' part of the values, code times step, comes to in each row: what the rounding of the weights is of."""
+    out, starts, group = torch.zeros(a["q"].shape, dtype=torch.float64, device="cuda"), a["starts"].tolist(), a["q"].shape[1] // a["k"].shape[1]
+    for b, n in enumerate(a["lengths"].tolist()):
+        j = torch.arange(n, device="cuda")
+        slots, i = a["table"][b].long()[j // a["page"]] * a["page"] + j % a["page"], torch.arange(n - starts[b + 1] + starts[b], n, device="cuda")
+        seen = (j[None] <= i[:, None]) & ((j[None] > i[:, None] - window) if window else True)
+        for h in range(a["q"].shape[1]):
+            code, step, low = held(a["k"][slots, h // group])
+            z = a["q"][starts[b]:starts[b + 1], h].double() @ (code * step + low).t() * scale
+            code, step, _ = held(a["v"][slots, h // group])
+            out[starts[b]:starts[b + 1], h] = torch.softmax(torch.where(seen, z, -INF), dim=1) @ (code * step)
+    return out
+
+
+# The weights of an fp16 cache are the sum of two 16-bit numbers, and within 2^-22 (one of them: 2^-11).  Tokens by twos have the same key and opposite values, of which nothing is left but what 4 bits make
+# of them, while the codes' parts of both add up to 15 steps; rows see few, so that the bounds of sums and scores are small beside 2^-12 of that
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64])
+@pytest.mark.parametrize("lengths,fresh,Hq,Hk,longest,window", [([4, 6, 8, 12] * 12, [1] * 48, 32, 8, None, None), ([4, 6, 8, 12] * 12, [1] * 48, 32, 4, None, None), ([4, 6, 8, 12] * 12, [4, 1, 5, 12] * 12, 16, 2, None, None),
+                                                                ([300, 800, 20], [3, 1, 20], 4, 2, None, 8), ([4, 8, 300, 6] * 8, [1] * 32, 16, 4, 16, 8), ([250, 390, 170], [240, 390, 150], 64, 64, None, 6)])
+def test_attend_fp16_weights_in_two_parts(lengths, fresh, Hq, Hk, longest, window, D):
+    a = make_attend(lengths, fresh, Hq, Hk, D, 16, "fp16", seed=D, q_scale=0.1)
+    k, v = a["k"].clone(), a["v"].clone()
+    k[1::2], v[1::2] = k[::2], -v[::2]
+    a = fill(a | dict(k=k, v=v), 16)
+    scale = D ** -0.5
+    want, lim, real = attend_exact(a, scale, window)
+    one, two = 2.0 ** -11, 2.0 ** -21
+    lim = lim - (one - two) * (1 + half("fp16")) * codes_part(a, scale, window)
+    got = ops.kv4_attention(a["q"], a["cache"], a["table"], a["lengths"], a["starts"], window=window, longest=longest)
+    off = (got.double() - want).abs()[real]
+    assert bool((off <= lim[real]).all()), f"off by {(off / lim[real]).max().item():.2f} of what is allowed"

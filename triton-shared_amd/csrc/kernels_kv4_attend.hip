@@ -440,9 +440,11 @@ __global__ __launch_bounds__(256, W > 4 || OWN == OWN_ROWS || (!BF16 && W == 4 &
           u32 w[4], rest[4];
           for (int i = 0; i < 4; i++) {
             const float a = e[0][i] * st[0][i], b = J == 1 ? dpp_moved<0x104>(a) : e[J - 1][i] * st[J - 1][i];  // (row_shl 4)
-            const tts_gemm_device::f16x2 pair = {(_Float16)a, (_Float16)b};
-            w[i] = __builtin_bit_cast(u32, pair);
+            w[i] = fp16_pair(a, b);
             if constexpr (!BF16) {
+              // (of the operand's own halves: made a second time, from the product without its rounding, they may be the next ones)
+              asm("" : "+v"(w[i]));
+              const tts_gemm_device::f16x2 pair = __builtin_bit_cast(tts_gemm_device::f16x2, w[i]);
               const float ra = __builtin_fmaf(e[0][i], st[0][i], -(float)pair[0]);
               rest[i] = fp16_pair(ra, J == 1 ? dpp_moved<0x104>(ra) : __builtin_fmaf(e[J - 1][i], st[J - 1][i], -(float)pair[1]));
             }
