@@ -1273,3 +1273,17 @@ def test_attend_fp16_weights_in_two_parts(lengths, fresh, Hq, Hk, longest, windo
     got = ops.kv4_attention(a["q"], a["cache"], a["table"], a["lengths"], a["starts"], window=window, longest=longest)
     off = (got.double() - want).abs()[real]
     assert bool((off <= lim[real]).all()), f"off by {(off / lim[real]).max().item():.2f} of what is allowed"
+
+
+# Prompts beside single tokens: in one call, and in two with the rows, lengths, tables and starts of each
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hk", [(8, 2), (64, 32)])
+def test_attend_prompts_and_single_tokens_in_one_call_and_in_two(Hq, Hk):
+    lengths, fresh = [700, 300, 5000, 40, 1, 2200], [700, 130, 1, 1, 1, 1]
+    a = make_attend(lengths, fresh, Hq, Hk, 64, seed=Hq)
+    check_attend(a)
+    prompts, singles = slice(0, 2), slice(2, 6)
+    for part in (prompts, singles):
+        first, behind = sum(fresh[:part.start]), sum(fresh[:part.stop])
+        x = a | dict(q=a["q"][first:behind], table=a["table"][part], lengths=a["lengths"][part], starts=a["starts"][part.start:part.stop + 1] - first)
+        check_attend(x, longest=max(lengths[part]))
