@@ -192,14 +192,13 @@ tts_status tts_kv4_read(const tts_tensor *cache, const tts_tensor *slots, const 
 
 /* Attention over the cache.  q [T, Hq, D], out the same (it may be q), Hq a multiple of Hk: head h reads the cache's head h / (Hq / Hk).  Rows starts[b] .. starts[b + 1] - 1 of q
  * are the last tokens of request b, which has lengths[b] tokens in the cache, in the pages table[b] (M columns, places for less than 2^30 tokens; starts [B + 1], lengths [B], table
- * [B, M] i32); the one at
- * position i sees tokens j <= i, with a window (not 0) i - window < j, whose page is in the table and in [0, pages).  Where starts[B] is past T, the rows that there are have the positions
- * that page_slots gives them.
+ * [B, M] i32); the one at position i sees tokens j <= i, with a window (not 0) i - window < j, whose page is in the table and in [0, pages).  Where starts[B] is past T, the rows that
+ * there are have the positions that page_slots gives them.
  *   out = sum over j of e^(z_j) v_j / sum of e^(z_j),  z_j = scale * q . k_j;  zeros for a row that sees none; rows of no request (before starts[0], behind starts[B])
  * are not written, or zeros if `clear`.
- * A row sees nothing of what others see alone: a NaN in a token's key or value reaches the rows that see it.  Scores, sums and statistics are held in 32 bits, e^z times a
+ * A row sees nothing of what others see alone: a NaN in a token's key or value reaches the rows that see it, and the largest values of tokens that it does not see leave it as it is.  Scores, sums and statistics are held in 32 bits, e^z times a
  * value's step in fp16 (2^-11 of it; of an fp16 cache as the sum of two of them, 2^-22), but for 2^-34 of the largest step so far among the tokens that it sees, q as it is but for
- * 2^-34 of its largest element.  A row whose largest element times the scale is not finite in 32 bits may be NaN.
+ * 2^-34 of its largest element, or 2^-147.   A row whose largest element times the scale is not finite in 32 bits may be NaN.
  * longest: no request has more tokens than that (0: as many as the table has places for); the number of workgroups follows it, and results do not depend on it but for the order of sums.  */
 tts_status tts_kv4_attention_workspace(const tts_tensor *q, const tts_tensor *cache, const tts_tensor *table, int window, int64_t longest, size_t *bytes);
 tts_status tts_kv4_attention(const tts_tensor *q, const tts_tensor *cache, const tts_tensor *table, const tts_tensor *lengths, const tts_tensor *starts, double scale, int window,

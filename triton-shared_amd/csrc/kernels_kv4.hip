@@ -3,8 +3,8 @@
 // what it then stands for is code * step + lowest.  A head whose range is not finite in 32 bits (it holds a NaN or an infinity) gets a step of NaN.
 // The 16 bits of step and lowest value are the format's: lowest is an element, exactly, and the rounding of step moves what the highest code stands for by 15 / 2 of a step's last place,
 // a thirtieth of a step in bf16.
-// What bounds them, 16384 tokens of 8 heads of 128: writing 23.8 us, 3.5 TB/s, by some 17 instructions an element; reading 19.5 us, 4.3 TB/s, by memory (at a copy's rate
-// 17 each).  64 tokens: 3.0 and 2.4 us, a launch.
+// What bounds them, 16384 tokens of 8 heads of 128: writing 24.9 us, 3.4 TB/s, by some 17 instructions an element (14 to 15 us of issue) behind loads that nothing
+// hides, since a lane asks for all it has and then computes; reading 19.7 us, 4.3 TB/s, by memory (at a copy's rate 17 each).  64 tokens: 3.0 and 2.5 us, a launch.
 #include <algorithm>
 
 #include "cache_ops.h"
@@ -146,7 +146,7 @@ hipError_t write_n(const Kv4RowsParams &p, hipStream_t s) {
   if (p.cache.dim <= 128) return go<T>(p, 16 / N, s, kv4_write_kernel<T, 16 / N, N>);
   return go<T>(p, 32 / N, s, kv4_write_kernel<T, 32 / N, N>);
 }
-// Of many heads a lane takes 32 elements of one, so that what is done once per lane counts less (16384 tokens of 8 heads of 128: 23.8 us, with 8 elements 30.5); of few
+// Of many heads a lane takes 32 elements of one, so that what is done once per lane counts less (16384 tokens of 8 heads of 128, side by side: 23.8 us, with 8 elements 30.5); of few
 // 8, for a shorter chain (64 tokens: 3.0 us, with 32 elements 4.0; 700: 3.9 and 4.2).
 template <class T>
 hipError_t write_as(const Kv4RowsParams &p, hipStream_t s) {

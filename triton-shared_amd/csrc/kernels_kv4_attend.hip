@@ -7,6 +7,8 @@
 // 2^-4 of itself.  q goes in as fp16 times a power of two per row that takes its largest element to [2^13, 2^14): exactly, but for 2^-34 of that element.
 // p_j a'_j goes in as fp16, times a power of two per row that takes the largest a' that it has seen so far to [2^13, 2^14) and 2^-4 for every second token: within 2^-11 of it, less than the rounding of a
 // bf16 output (2^-8); where the output is fp16 too, as the sum of two (2^-22); and within 2^-34 of the largest a'.  All sums and the statistics are in 32 bits.
+// (The sum of two for bf16 as well: 64 ragged requests 36.5 us (one 35.3), 5 tokens each of 16 requests 30.4 (25.7), prompts 258 (221), for errors against the exact result of 1.71e-3 instead of 1.73e-3, of
+// which 1.71e-3 is the output's rounding.)
 //
 // A wavefront takes blocks of 64 tokens.  Keys: lane (m, g) = (lane % 16, lane / 16) loads a quarter g of token m of each of four tiles, which is the
 // left operand of  scores[token][row];  so a lane gets the scores of tokens 4 g .. 4 g + 3 of each tile for row m, and what it makes of them is the right
@@ -15,9 +17,9 @@
 // What bounds it, dim 128 and 8 heads of the cache, bf16 (a copy of 1 GiB runs at 5.0 TB/s, a 16-bit matrix product of 8192^3 at 1.19 PFLOP/s):
 //   64 requests of 100 .. 8192 tokens (118 MB): 35 us in a graph, of which joining the slices 4: 3.8 TB/s while it runs.  The chain before a workgroup's first block, 3.4 us where it is alone
 //     (lengths, table and codes, one after another), and its last steps are not hidden by others: there is one round of workgroups, and more of them cost as much as they hide.
-//   2 of 131072, 64 heads of q: 35 us, 29 + 6: 4.4 TB/s.   1 of 4000: 11.4 us, 8.3 + 3.2: the chains.
-//   4 x 1024 rows behind up to 4096 tokens: 219 us, 602 TFLOP/s: the vector instructions, some 570 to 64 matrix instructions in a block of 32 rows (160 of them unpack codes, 350 are the softmax); they
-//     fill two thirds of the cycles, the matrix instructions a quarter, and two wavefronts per SIMD, which is what 250 registers allow, hide little of one behind the other.
+//   2 of 131072, 64 heads of q: 35 us, 29 + 6: 4.4 TB/s.   1 of 4000: 11.8 us, 8.5 + 3.3: the chains.
+//   4 x 1024 rows behind up to 4096 tokens: 221 us, 598 TFLOP/s (of an fp16 cache 258, 512): the vector instructions, some 570 to 64 matrix instructions in a block of 32 rows (160 of them unpack codes, 350 are the softmax); they
+//     fill two thirds of the cycles, the matrix instructions a quarter, and two wavefronts per SIMD, which is what 234 registers allow, hide little of one behind the other.
 #include <algorithm>
 #include <type_traits>
 
@@ -639,15 +641,17 @@ hipError_t launch_as(const AttendParams &p, hipStream_t s) {
 }  // namespace
 
 // Which kernel, and how many workgroups.  Both sides of each rule as measured, us a call in a graph, dim 128 and 8 heads of the cache where nothing else is said:
-// * Rows of their own for each wavefront where a request has 128 and more on average and they make 384 workgroups: 64 requests of 256 rows 405 (shared rows 537), 16 of 512 217
-//   (267), but 16 of 256 166 (162) and 4 of 1024 140 (119): fewer workgroups do not fill the device, and the tokens are what is left to divide.
-// * Heads of their own for each wavefront where there are 4 requests and heads for each token of the longest: 256 requests of 250 17.4 (shared blocks 27.1), 128 of up to 60 7.4 (12.6),
-//   512 of up to 1000 45.5 (58.9), but 64 of up to 250 10.4 (8.3), 128 of up to 1000 25.4 (19.0); between them 256 of up to 1000 27.8 (29.0): what a workgroup does before and after
+// * Rows of their own for each wavefront where a request has 128 and more on average and they make 384 workgroups: 64 requests of 256 rows 394 (shared blocks 466), 16 of 512 209
+//   (220), but 16 of 256 158 (120) and 4 of 1024 132 (95): fewer workgroups do not fill the device, and the tokens are what is left to divide.
+// * Heads of their own for each wavefront where there are 4 requests and heads for each token of the longest: 256 requests of 250 17.2 (shared blocks 27.1), 128 of up to 60 7.7 (12.8), 512 of up to 60
+//   21.4 (42.5), 512 of up to 1000 44.5 (59.8), but 64 of up to 250 10.7 (8.4), 128 of up to 1000 26.3 (19.2); between them 256 of up to 1000 28.8 (30.3, and by the rule shared): what a workgroup does before and after
 //   its blocks counts for four heads, and a head's blocks come one after another.
-// * Tiles of 4 or 8 rows where a request has no more: 16 requests of 4000 tokens, 4 rows 21.4 (tiles of 8 21.9, of 16 22.7), 8 rows 22.4 (of 16 23.3, of 4 30.6).
-// * Slices, of 512 workgroups beyond the tiles', where the longest request has more than 1024 tokens and 6 for each tile: 64 requests of up to 8192 34.8 (none: 50.7),
-//   128 of up to 8000 71.7 (76.1), one of 1500 11.7 (13.2), but 128 of 4000 120.9 (113.5), 256 of up to 2000 63.5 (41.4), one of 600 11.4 (9.3): the second kernel, and what a
+// * Tiles of 4 or 8 rows where a request has no more: 16 requests of 4000 tokens, 4 rows 21.3 (tiles of 8 21.6, of 16 22.6), 8 rows 21.4 (of 16 22.9, of 4 29.2).
+// * Slices, of 512 workgroups beyond the tiles', where the longest request has more than 1024 tokens and 6 for each tile: 64 requests of up to 8192 35.2 (none: 47.5),
+//   128 of up to 8000 65 (72), one of 1500 11.8 (12.8), but 128 of 4000 112 (109), 256 of up to 2000 53.0 (39.0), one of 600 11.6 (9.2): the second kernel, and what a
 //   workgroup does before its first block and behind its last.
+// All of them are batches of one number of new tokens for every request, and the average is all that the rules know: of others they may choose badly.  2048 rows of a prompt take 86 alone and 7 tokens of up
+// to 8192 19, in one call 252 (of up to 131072 136, in one call 3771: a wavefront with rows of its own walks all of their tokens); 64 single tokens 65, padded to 8192 rows 590.
 AttendPlan plan_attend(int64_t tokens, int requests, int heads, int kv_heads, int dim, int64_t longest, int window) {
   AttendPlan plan = {};
   const int64_t group = heads / kv_heads, rows = (tokens + requests - 1) / std::max(requests, 1) * group;  // of a request, on average

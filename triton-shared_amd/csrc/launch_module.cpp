@@ -408,7 +408,7 @@ PyObject *op_page_slots(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const tts_tensor *p[10] = {};
   for (int i = 0; i < 5; i++) p[i] = o.describe(a[i], t[i]);
   if (!o.ok || !p[0] || p[0]->rank != 2) return not_ordinary();
-  // the five results lie in one buffer (five of their own: 15.0 us a call; so 10)
+  // the five results lie in one buffer (five of their own cost a call 5 us more)
   const int64_t requests = t[0].shape[0], sizes[5] = {rows, rows, rows, requests + 1, 1};
   tts_tensor all;
   Ref buffer(o.make(a[0], -1, 3 * rows + requests + 2, g_ops.dtypes[TTS_I32], all)), split(Py_BuildValue("(LLLLL)", (long long)rows, (long long)rows, (long long)rows, (long long)requests + 1, 1LL));
