@@ -7,8 +7,8 @@
 // 2^-4 of itself.  q goes in as fp16 times a power of two per row that takes its largest element to [2^13, 2^14): exactly, but for 2^-34 of that element.
 // p_j a'_j goes in as fp16, times a power of two per row that takes the largest a' that it has seen so far to [2^13, 2^14) and 2^-4 for every second token: within 2^-11 of it, less than the rounding of a
 // bf16 output (2^-8); where the output is fp16 too, as the sum of two (2^-22); and within 2^-34 of the largest a'.  All sums and the statistics are in 32 bits.
-// (The sum of two for bf16 as well: 64 ragged requests 36.5 us (one 35.3), 5 tokens each of 16 requests 30.4 (25.7), prompts 258 (221), for errors against the exact result of 1.71e-3 instead of 1.73e-3, of
-// which 1.71e-3 is the output's rounding.)
+// (The sum of two for bf16 as well: 64 ragged requests 36.5 us (one 35.3), 5 tokens each of 16 requests 30.4 (25.7), prompts, as fp16 has them, 258 (221),
+// for errors against the exact result of 1.71e-3 instead of 1.73e-3, of which 1.71e-3 is the output's rounding.)
 //
 // A wavefront takes blocks of 64 tokens.  Keys: lane (m, g) = (lane % 16, lane / 16) loads a quarter g of token m of each of four tiles, which is the
 // left operand of  scores[token][row];  so a lane gets the scores of tokens 4 g .. 4 g + 3 of each tile for row m, and what it makes of them is the right
